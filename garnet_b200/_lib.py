@@ -63,6 +63,15 @@ def _declare(L: ctypes.CDLL) -> None:
     L.garnet_b200_w4a16_list_create_ex.argtypes = [vp, i, i, c.POINTER(vp)]
     L.garnet_b200_attention_decode_workspace.argtypes = [vp, i, c.POINTER(sz)]
     L.garnet_b200_attention_decode.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i, c.c_uint, vp]
+    L.garnet_b200_attention_chunk_workspace.argtypes = [vp, i, c.POINTER(sz)]
+    L.garnet_b200_attention_chunk.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i, i, i, u, vp]
+    L.garnet_b200_log_probs.argtypes = [vp, i, c.c_int64, vp, i, i, i, c.c_float, vp, vp, vp, vp, vp, u, vp]
+    L.garnet_b200_cache_workspace.argtypes = [vp, i, c.POINTER(sz)]
+    L.garnet_b200_cache_extend.argtypes = [vp, vp, vp, vp, vp, vp, vp, i, vp, sz, vp]
+    L.garnet_b200_cache_fork.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, sz, vp]
+    L.garnet_b200_cache_free.argtypes = [vp, vp, vp, vp, vp, i, vp]
+    L.garnet_b200_cache_compact.argtypes = [vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.garnet_b200_cache_copy_pages.argtypes = [vp, vp, vp, vp, vp, i, vp]
     L.garnet_b200_embedding_gather.argtypes = [vp, vp, vp, i, i, i, c.c_uint, vp]
     L.garnet_b200_argmax_bf16.argtypes = [vp, vp, i, i, c.c_uint, vp]
     L.garnet_b200_safetensors_open.argtypes = [c.c_char_p, c.POINTER(vp)]
@@ -148,3 +157,16 @@ def stream_ptr() -> int:
     """Handle of the current stream of the current device.  Asked for by its raw handle: building a
     torch.cuda.Stream object for it took 3.2 us of a call whose kernel runs 6 us."""
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def on_device(t, name: str, dtype=None, shape=None):
+    """`t` when it is a contiguous CUDA tensor on the current device, of the given type and shape (None in a shape: any extent)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} must be a tensor on the current CUDA device")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
+    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape))):
+        raise ValueError(f"{name} must have the shape {tuple('any' if w is None else w for w in shape)}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t

@@ -23,11 +23,12 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from typing import NamedTuple, Optional
 
 import numpy as np
 import torch
 
-from ._lib import check, lib, stream_ptr
+from ._lib import BF16, FP16, FP32, check, lib, on_device, stream_ptr
 from .linear import GlueList, W4A16Linear
 
 
@@ -85,6 +86,47 @@ class PagedAttention:
         return out
 
 
+class ChunkAttention:
+    """garnet_b200_attention_chunk with its workspace: attention of a chunk of new tokens of each of several sequences - a prompt, a
+    further piece of one, drafted tokens to verify - which PagedAttention does for one token each.  `run` takes up to `max_tokens` rows
+    of `qkv` [rows, (q_heads + 2 kv_heads) * 128] bf16; sequence b has the rows row_starts[b] .. row_starts[b + 1] - 1 (int32 [batch + 1])
+    at the slots positions[b], positions[b] + 1, ... of page_tables[b].  The object's workspace serves one call at a time."""
+
+    def __init__(self, cfg: DecoderConfig, max_tokens: int, max_context: int, max_logical_pages: int, rope_positions: int):
+        self.opt = AttentionOptions(abi=1, struct_size=ctypes.sizeof(AttentionOptions), q_heads=cfg.q_heads, kv_heads=cfg.kv_heads,
+                                    head_dim=cfg.head_dim, page_size=cfg.page_size, max_logical_pages=max_logical_pages,
+                                    max_context=max_context, rope_positions=rope_positions, norm_eps=cfg.eps)
+        need = ctypes.c_size_t(0)
+        check(lib().garnet_b200_attention_chunk_workspace(ctypes.byref(self.opt), max_tokens, ctypes.byref(need)))
+        self.ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+
+    def run(self, qkv, q_norm_w, k_norm_w, cos, sin, key_pages, value_pages, page_tables, positions, row_starts, out, pdl: bool = False):
+        o, bf, i32 = self.opt, torch.bfloat16, torch.int32
+        on_device(qkv, "qkv", bf, (None, (o.q_heads + 2 * o.kv_heads) * o.head_dim))
+        batch, rows = positions.numel(), qkv.shape[0]
+        for w, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
+            on_device(w, name, bf, (o.head_dim,))
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            on_device(t, name, torch.float32, (None, o.head_dim // 2))
+            if t.shape[0] < o.rope_positions:
+                raise ValueError(f"{name} has fewer than {o.rope_positions} rows")
+        on_device(key_pages, "key_pages", bf, (None, o.page_size, o.kv_heads, o.head_dim))
+        on_device(value_pages, "value_pages", bf, tuple(key_pages.shape))
+        on_device(page_tables, "page_tables", i32, (batch, o.max_logical_pages))
+        on_device(positions, "positions", i32, (batch,))
+        on_device(row_starts, "row_starts", i32, (batch + 1,))
+        on_device(out, "out", bf, (rows, o.q_heads * o.head_dim))
+        if self.ws.device != qkv.device:
+            raise ValueError("the workspace is on another device than the rows")
+        if batch and rows:
+            check(lib().garnet_b200_attention_chunk(ctypes.byref(o), qkv.data_ptr(), q_norm_w.data_ptr(), k_norm_w.data_ptr(),
+                                                    cos.data_ptr(), sin.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
+                                                    page_tables.data_ptr(), positions.data_ptr(), row_starts.data_ptr(), out.data_ptr(),
+                                                    self.ws.data_ptr(), self.ws.numel(), batch, rows, key_pages.shape[0],
+                                                    1 if pdl else 0, stream_ptr()))
+        return out
+
+
 def embedding_gather(table, ids, out, pdl: bool = False):
     check(lib().garnet_b200_embedding_gather(table.data_ptr(), ids.data_ptr(), out.data_ptr(), ids.numel(), table.shape[1],
                                              table.shape[0], 1 if pdl else 0, stream_ptr()))
@@ -95,6 +137,39 @@ def argmax_bf16(logits, out, pdl: bool = False):
     check(lib().garnet_b200_argmax_bf16(logits.data_ptr(), out.data_ptr(), logits.shape[0], logits.shape[1], 1 if pdl else 0,
                                         stream_ptr()))
     return out
+
+
+class LogProbs(NamedTuple):
+    log_probs: Optional[torch.Tensor]        # [rows] fp32, None without targets
+    ranks: Optional[torch.Tensor]            # [rows] int32, None without targets
+    entropy: torch.Tensor                    # [rows] fp32
+    top_log_probs: torch.Tensor              # [rows, top_k] fp32
+    top_ids: torch.Tensor                    # [rows, top_k] int32
+
+
+_LOGIT_KIND = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32}
+
+
+def log_probs(logits, targets=None, top_k: int = 0, temperature: float = 1.0, pdl: bool = False) -> LogProbs:
+    """Log probability and rank of the token targets[r] (int32) under softmax(logits[r] / temperature), the row's entropy and its top_k
+    tokens, for logits [rows, vocab] of fp32, bf16 or fp16 (rows may lie further apart than vocab)."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _LOGIT_KIND:
+        raise ValueError("log_probs needs logits [rows, vocab] of fp32, bf16 or fp16")
+    rows, vocab = logits.shape
+    stride = logits.stride(0) if rows > 1 else vocab
+    if not logits.is_cuda or logits.device.index != torch.cuda.current_device() or (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+        raise ValueError("log_probs needs rows of neighbouring values on the current CUDA device")
+    if targets is not None:
+        on_device(targets, "targets", torch.int32, (rows,))
+    f32, i32 = dict(dtype=torch.float32, device=logits.device), dict(dtype=torch.int32, device=logits.device)
+    r = LogProbs(None if targets is None else torch.empty(rows, **f32), None if targets is None else torch.empty(rows, **i32),
+                 torch.empty(rows, **f32), torch.empty(rows, max(0, top_k), **f32), torch.empty(rows, max(0, top_k), **i32))
+    if rows:
+        ptr = lambda t: None if t is None or not t.numel() else t.data_ptr()   # noqa: E731
+        check(lib().garnet_b200_log_probs(logits.data_ptr(), _LOGIT_KIND[logits.dtype], stride, ptr(targets), rows, vocab, top_k, temperature,
+                                          ptr(r.log_probs), ptr(r.ranks), ptr(r.entropy), ptr(r.top_log_probs), ptr(r.top_ids),
+                                          1 if pdl else 0, stream_ptr()))
+    return r
 
 
 class DecodeStep:

@@ -325,12 +325,97 @@ int garnet_b200_attention_decode(const garnet_b200_attention_options* options, c
                                  void* d_value_pages, const int* d_page_tables, const int* d_positions, void* d_out,
                                  void* d_workspace, size_t workspace_bytes, int batch, unsigned flags, void* stream);
 
+/* Attention of a chunk of new tokens of each of `batch` sequences: a prompt, a further piece of one, drafted tokens to verify.  The
+ * rows of the sequences lie one after the other: sequence b has the rows row_starts[b] .. row_starts[b + 1] - 1 of d_qkv (int32
+ * [batch + 1], ascending, within 0 .. tokens; a sequence may have none), its first row the slot d_positions[b], the next rows the
+ * slots behind it.  Every row is treated as by garnet_b200_attention_decode - head norms, RoPE, k and v appended to the cache - and
+ * sees the slots up to its own, those that the call itself appends included.  `tokens` is the number of rows of d_qkv
+ * [tokens, (q_heads + 2 kv_heads) * 128] and d_out [tokens, q_heads * 128] (bf16); rows of no sequence are left as they are.
+ *   - A row whose slot is negative, or not below max_context, appends nothing and comes out as zeros.
+ *   - Slots whose page is not one of the `physical_pages` of the cache are not written and not seen; a row that sees none is zeros.
+ *   - What the cache holds behind a sequence's last slot does not matter (NaN and infinities included).
+ *   - Pages that hold the slots of new rows belong to one sequence each; full pages before them may be shared.
+ *   - q_heads / kv_heads at most 128.
+ * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned) needs no clearing and holds nothing
+ * between calls; calls that overlap on the GPU need one each.  flags bit 0: programmatic dependent launch.  No allocation, no
+ * synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step
+ * (src/cuda/text_kv_attention_kernel.cu:640-840). */
+int garnet_b200_attention_chunk_workspace(const garnet_b200_attention_options* options, int tokens, size_t* bytes);
+int garnet_b200_attention_chunk(const garnet_b200_attention_options* options, const void* d_qkv, const void* d_q_norm_weight,
+                                const void* d_k_norm_weight, const float* d_rope_cos, const float* d_rope_sin, void* d_key_pages,
+                                void* d_value_pages, const int* d_page_tables, const int* d_positions, const int* d_row_starts,
+                                void* d_out, void* d_workspace, size_t workspace_bytes, int batch, int tokens, int physical_pages,
+                                unsigned flags, void* stream);
+
 /* out[b, :] = table[ids[b], :] (bf16 [vocab, hidden]; ids outside the table are clamped). */
 int garnet_b200_embedding_gather(const void* d_table, const int* d_ids, void* d_out, int batch, int hidden, int vocab,
                                  unsigned flags, void* stream);
 
 /* out[b] = index of the largest of logits[b, :vocab] (bf16), the lowest index among equals. */
 int garnet_b200_argmax_bf16(const void* d_logits, int* d_out, int batch, int vocab, unsigned flags, void* stream);
+
+/* Log probabilities of rows of logits z [rows, vocab] (dtype GARNET_B200_BF16, _FP16 or _FP32, rows `row_stride` elements apart)
+ * under p = softmax(z / temperature):
+ *   d_log_probs[r]  log p(d_targets[r])        d_ranks[r]  1 + how many logits are larger than the target's
+ *   d_entropy[r]    -sum p log p               d_top_ids / d_top_log_probs [rows, top_k]: the largest logits in descending order,
+ *                                              the lowest index first among equals
+ * (fp32 and int32).  d_targets, d_log_probs and d_ranks are given together or all NULL, d_entropy may be NULL, the top arrays are NULL
+ * when top_k is 0; top_k is at most 32 and at most vocab.
+ *   - A target outside 0 .. vocab - 1 (a row without one) gets log probability 0 and rank 0.
+ *   - Logits of -inf have probability 0 and add nothing; a row of nothing else has log probabilities -inf and entropy 0.
+ *   - A NaN or +inf among a row's logits makes its log probabilities and entropy NaN.  NaN is no alternative: where a row has fewer than
+ *     top_k others, the ids behind them are -1.
+ * Sums are fp32; no workspace, no allocation, no synchronisation; the results do not depend on timing.  flags bit 0: programmatic
+ * dependent launch.  The reference's sampler stops at the top token (src/cuda/logits_sampler_kernel.cu). */
+int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, const int* d_targets, int rows, int vocab, int top_k,
+                          float temperature, float* d_log_probs, int* d_ranks, float* d_entropy, float* d_top_log_probs, int* d_top_ids,
+                          unsigned flags, void* stream);
+
+/* ---- pages of the KV cache --------------------------------------------------------
+ * Hands the pages of a paged cache out to sequences, shares them between forked sequences, takes them back and moves them
+ * together, on the device: a captured step can be followed by a fork without a trip to the host.  The state is three int32 arrays
+ * that the caller owns: d_page_tables [sequences, max_logical_pages] (what the attention calls read; -1 where a row has no page),
+ * d_lengths [sequences] (positions that a sequence holds, in its first ceil(length / page_size) pages) and
+ * d_refcounts [physical_pages] (table entries that refer to the page; 0 = free).  An empty pool is -1, 0 and 0.  A host that pins a
+ * page adds one to its count.  Lists (sequence numbers, token counts, pages) are int32 arrays on the device.  The outcome is a
+ * function of state and lists alone.  d_status[i]: GARNET_B200_OK, _INVALID_VALUE (entry i is refused) or _OUT_OF_MEMORY (too few free
+ * pages: from the first entry on that does not get its pages, entries that need one get none; nothing is changed for them).
+ * key_pages / value_pages are host arrays of `layers` device pointers (16-byte aligned, read during the call), the cache of each layer
+ * [physical_pages][page_size][token_bytes].  Calls on one pool are ordered by their stream.  The workspace
+ * (garnet_b200_cache_workspace for lists of up to `count` entries, 256-byte aligned) holds nothing between calls.  The reference keeps
+ * its page pool on the host (src/runtime/). */
+typedef struct garnet_b200_cache_options {
+    int abi;                /* GARNET_B200_ABI */
+    int struct_size;        /* sizeof(garnet_b200_cache_options) */
+    int layers;             /* up to 128 */
+    int physical_pages;     /* pages of a layer's cache */
+    int page_size;          /* positions per page */
+    int token_bytes;        /* bytes of a position's K (and of its V) in a layer: kv_heads * head_dim * 2; a multiple of 16 */
+    int sequences;          /* rows of the page table */
+    int max_logical_pages;  /* columns of the page table */
+} garnet_b200_cache_options;
+int garnet_b200_cache_workspace(const garnet_b200_cache_options* options, int count, size_t* bytes);
+/* Sequence d_sequences[i] grows by d_tokens[i] positions and gets the lowest free pages that these need.  Refused: a sequence that an
+ * earlier entry names, a number outside the tables, a negative count, more positions than a row of the table has room for. */
+int garnet_b200_cache_extend(const garnet_b200_cache_options* options, int* d_page_tables, int* d_lengths, int* d_refcounts,
+                             const int* d_sequences, const int* d_tokens, int* d_status, int count, void* d_workspace,
+                             size_t workspace_bytes, void* stream);
+/* Sequence d_children[i] becomes a copy of d_parents[i]: it refers to the parent's full pages, and the positions in the parent's last,
+ * partial page are copied to the lowest free page, in every layer.  Refused: a child that holds positions or that an earlier entry
+ * names, a parent that is a child of any entry, numbers outside the tables. */
+int garnet_b200_cache_fork(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages, int* d_page_tables,
+                           int* d_lengths, int* d_refcounts, const int* d_parents, const int* d_children, int* d_status, int count,
+                           void* d_workspace, size_t workspace_bytes, void* stream);
+/* The sequences give their pages back and are empty (numbers outside the tables are passed over, a sequence named twice is freed once). */
+int garnet_b200_cache_free(const garnet_b200_cache_options* options, int* d_page_tables, int* d_lengths, int* d_refcounts,
+                           const int* d_sequences, int count, void* stream);
+/* Moves pages so that the live ones (reference count > 0) are pages 0 .. live - 1, as few as that takes: the i-th live page with a number
+ * of `live` or more goes to the i-th free page below it; tables and counts follow.  d_live[0] = live. */
+int garnet_b200_cache_compact(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages, int* d_page_tables,
+                              int* d_refcounts, int* d_live, void* d_workspace, size_t workspace_bytes, void* stream);
+/* Copies page d_src[i] to page d_dst[i] in every layer, as if one pair after the other; pairs with a page outside the cache are passed over. */
+int garnet_b200_cache_copy_pages(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages, const int* d_src,
+                                 const int* d_dst, int count, void* stream);
 
 /* ---- the rest of a gpt-oss decoder layer -----------------------------------------
  * The operators around the MoE that the reference's plugin also carries (GptOssOptions kinds 0, 1,
