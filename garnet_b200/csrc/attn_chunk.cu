@@ -3,66 +3,15 @@
 // 1 / sqrt(128) (src/backends/tensorrt/trt_builder.cpp:7565-7726, src/cuda/text_kv_attention_kernel.cu:640-840).
 //
 // Two launches: attn_chunk_rows_kernel normalises and rotates q and k of every row, appends k and v to the cache and leaves the
-// queries in the workspace, a kv head's rows together; attn_chunk_kernel walks the context of every row.
+// queries in the workspace, a kv head's rows together; the kernel of attn_chunk_tc.cu does the attention.
 #include <algorithm>
 #include <cstdint>
 
-#include "common.cuh"
+#include "attn_chunk.cuh"
 
 namespace gb200 {
 
 namespace {
-
-constexpr int kChDim = 128;
-
-struct Chunk {
-    const __nv_bfloat16* qkv;        // [tokens, (q_heads + 2 kv_heads) * 128]
-    const __nv_bfloat16* q_norm_w;   // [128]
-    const __nv_bfloat16* k_norm_w;
-    const float* rope_cos;           // [positions, 64]
-    const float* rope_sin;
-    __nv_bfloat16* keys;             // [physical pages][page size][kv heads][128]
-    __nv_bfloat16* values;
-    const int* tables;               // [batch, width]
-    const int* positions;            // [batch]: slot of a sequence's first new row
-    const int* row_starts;           // [batch + 1]
-    __nv_bfloat16* out;              // [tokens, q_heads * 128]
-    __nv_bfloat16* queries;          // workspace: [kv head][token][q head of the group][128]
-    int batch, tokens, q_heads, kv_heads, page_size, width, physical_pages, max_context;
-    float eps;
-};
-
-// The sequence of a row, -1 where it has none.
-__device__ __forceinline__ int chunk_sequence(const Chunk& p, int row)
-{
-    int lo = 0, hi = p.batch;   // the last b with row_starts[b] <= row
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.row_starts[mid] <= row) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo < p.batch && p.row_starts[lo] <= row && row < p.row_starts[lo + 1] ? lo : -1;
-}
-// The slot of a row, -1 where it appends and sees nothing.
-__device__ __forceinline__ int chunk_slot(const Chunk& p, int b, int row)
-{
-    const long long slot = (long long)p.positions[b] + (row - p.row_starts[b]);
-    return p.positions[b] >= 0 && slot < p.max_context ? int(slot) : -1;
-}
-// Offset of a slot's K and V of a head; -1 where it has no page.
-__device__ __forceinline__ long long chunk_cache_offset(const Chunk& p, int b, int slot, int head)
-{
-    const int page = p.tables[size_t(b) * p.width + slot / p.page_size];
-    if (page < 0 || page >= p.physical_pages) return -1;
-    return (((long long)page * p.page_size + slot % p.page_size) * p.kv_heads + head) * kChDim;
-}
-
-__device__ __forceinline__ float chunk_warp_sum(float v)
-{
-#pragma unroll
-    for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
-}
 
 // a cos + b sin with one rounding's error: the second product's own is added back.
 __device__ __forceinline__ float turned(float a, float cosine, float b, float sine)
@@ -124,44 +73,6 @@ __global__ void __launch_bounds__(256) attn_chunk_rows_kernel(const Chunk p)
         }
         to[lane] = lo, to[lane + 32] = hi;
     }
-}
-
-// One (row, q head) by one warp, slot after slot: running maximum and sum in fp32, four dims per lane.
-__device__ __forceinline__ void chunk_row(const Chunk& p, int b, int row, int head, int slot, int lane)
-{
-    const int group = p.q_heads / p.kv_heads, kv = head / group;
-    const uint2 qr = *(reinterpret_cast<const uint2*>(p.queries + ((size_t(kv) * p.tokens + row) * group + head % group) * kChDim) + lane);
-    const float q[4] = {__uint_as_float(qr.x << 16), __uint_as_float(qr.x & 0xffff0000u), __uint_as_float(qr.y << 16), __uint_as_float(qr.y & 0xffff0000u)};
-    float top = -INFINITY, sum = 0.f, o[4] = {};
-    for (int s = 0; s <= slot; ++s) {
-        const long long at = chunk_cache_offset(p, b, s, kv);
-        if (at < 0) continue;
-        const uint2 kr = *(reinterpret_cast<const uint2*>(p.keys + at) + lane), vr = *(reinterpret_cast<const uint2*>(p.values + at) + lane);
-        const float score = chunk_warp_sum(q[0] * __uint_as_float(kr.x << 16) + q[1] * __uint_as_float(kr.x & 0xffff0000u) +
-                                           q[2] * __uint_as_float(kr.y << 16) + q[3] * __uint_as_float(kr.y & 0xffff0000u)) * 0.08838834764831845f;
-        if (score == -INFINITY) continue;   // weight 0
-        const float next = fmaxf(top, score), old = top == next ? 1.f : expf(top - next), w = expf(score - next);
-        const float v[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u), __uint_as_float(vr.y << 16), __uint_as_float(vr.y & 0xffff0000u)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * old + w * v[i];
-        sum = sum * old + w;
-        top = next;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const __nv_bfloat162 r[2] = {__floats2bfloat162_rn(o[0] * inv, o[1] * inv), __floats2bfloat162_rn(o[2] * inv, o[3] * inv)};
-    *(reinterpret_cast<uint2*>(p.out + (size_t(row) * p.q_heads + head) * kChDim) + lane) = *reinterpret_cast<const uint2*>(r);
-}
-
-__global__ void __launch_bounds__(256) attn_chunk_kernel(const Chunk p)
-{
-    pdl_launch_dependents();
-    pdl_wait();
-    const int task = int(blockIdx.x) * 8 + int(threadIdx.x >> 5), lane = threadIdx.x & 31;
-    const int row = task / p.q_heads, head = task % p.q_heads;
-    if (row >= p.tokens) return;
-    const int b = chunk_sequence(p, row);
-    if (b < 0) return;
-    chunk_row(p, b, row, head, chunk_slot(p, b, row), lane);
 }
 
 int validate_chunk(const garnet_b200_attention_options* o)
@@ -230,6 +141,8 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
         return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: rows, cache pages, rope tables and output must be 16-byte aligned");
     if ((reinterpret_cast<uintptr_t>(d_q_norm_weight) | reinterpret_cast<uintptr_t>(d_k_norm_weight)) & 3)
         return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: the norm weights must be 4-byte aligned");
+    if ((long long)physical_pages * o->page_size > 0x7fff0000ll || (long long)tokens * o->q_heads > 0x7fff0000ll)
+        return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: more than 2^31 cache slots or query rows");
     Chunk p;
     p.qkv = static_cast<const __nv_bfloat16*>(d_qkv);
     p.q_norm_w = static_cast<const __nv_bfloat16*>(d_q_norm_weight);
@@ -245,8 +158,7 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     p.eps = o->norm_eps;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     GB_CUDA(chunk_launch(attn_chunk_rows_kernel, dim3(unsigned(tokens)), s, (flags & 1u) != 0, p));
-    GB_CUDA(chunk_launch(attn_chunk_kernel, dim3(unsigned(((long long)tokens * o->q_heads + 7) / 8)), s, true, p));
-    return GARNET_B200_OK;
+    return chunk_attention_launch(p, s);
 }
 
 }  // extern "C"

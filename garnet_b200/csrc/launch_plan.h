@@ -59,4 +59,21 @@ inline int oss_prefill_tiles(int batch, int kv_heads, int tokens, int tile_token
     return tokens > tile_tokens && batch * (long long)kv_heads * pairs >= kSmCount ? 2 : 1;
 }
 
+// Chunk attention (attn_chunk_tc.cu): tiles of 128 query rows per CTA, and CTAs of a cluster that share a tile's keys.  Two tiles where
+// that still gives every SM a CTA; one tile each otherwise, two CTAs to an SM, and the keys in 2, 4 or 8 shares as long as the CTAs run
+// at once and a share has two steps of 64 keys at the longest context.
+struct ChunkPlan {
+    int tiles, splits;
+};
+inline ChunkPlan chunk_plan(int batch, int kv_heads, int tokens, int tile_tokens, int max_context)
+{
+    const long long each = (tokens + batch - 1) / batch;   // rows of a sequence, were they all as long
+    const long long pairs = batch * ((each + 2 * tile_tokens - 1) / (2 * tile_tokens)) * kv_heads;
+    if (each > tile_tokens && pairs >= kSmCount * 3 / 4) return {2, 1};
+    const long long ctas = std::min<long long>(tokens, batch * ((each + tile_tokens - 1) / tile_tokens)) * kv_heads;
+    int splits = 1;
+    while (splits < 8 && ctas * splits * 2 <= 2 * kSmCount && max_context >= splits * 2 * 128) splits *= 2;
+    return {1, splits};
+}
+
 }  // namespace gb200

@@ -170,6 +170,15 @@ def test_many_sequences():
     Case(lens, [int(n) for n in r.randint(0, 150, 70)], 4, 2).check()
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,lens,starts,page_size", [
+    (16, 8, [130, 90, 1, 127, 128, 129, 64, 65, 260, 0, 33, 100, 77, 128], [0, 5, 300, 128, 127, 1, 64, 63, 0, 9, 500, 250, 1, 0], 16),
+    (18, 6, [90, 43, 85, 130, 84, 42, 41, 100, 100, 86, 129, 60, 70, 127, 3, 1, 88, 99, 47, 90], [20 * i for i in range(20)], 20),
+    (30, 30, [129, 257, 200, 255], [0, 100, 37, 1], 64)])
+def test_batches_that_fill_the_gpu(q_heads, kv_heads, lens, starts, page_size):
+    """Two tiles of query rows to a CTA."""
+    Case(lens, starts, q_heads, kv_heads, page_size=page_size, pad=2, seed=q_heads).check()
+
+
 def test_sharp_scores():
     """Scores of some hundreds: all weight on single positions, maxima that grow from tile to tile, rows whose largest score comes last."""
     c = Case([140], [400], 2, 1, seed=5)
