@@ -1,21 +1,39 @@
-// Log probabilities of given tokens, their ranks, entropies and the top alternatives of rows of logits.
+// Log probabilities of given tokens, their ranks, entropies and the top alternatives of rows of logits, in one pass over the logits.
 //
-//   z = x / temperature, m = max z, S = sum e^(z - m):   log p(t) = z_t - m - log S,   H = log S - sum e^(z - m) (z - m) / S,
-//   rank = 1 + #{x > x_t}.
+//   y = x log2(e) / T, a reference r near the row's maximum of y, S = sum 2^(y - r), W = sum 2^(y - r) (y - r):
+//   log p(t) = ln 2 ((y_t - r) - log2 S),  H = ln 2 (log2 S - W / S),  rank = 1 + #{x > x_t}.
 //
-// One CTA per row: the maximum, then the sums and the rank, then one pass over the row for every alternative.
-// Bound: HBM in principle (every logit once).
+// A row is cut into 1, 2, 4 or 8 parts, one CTA each, that meet through distributed shared memory.  The warps of a CTA take blocks of 1 KB in
+// turn: two 16-byte loads per lane, the block's maximum (NaN wins) by packed maxima and one warp reduction, which also says whether the
+// warp's reference has to grow (by more than 2^8, so that this is rare: S and W are rescaled then), then per value one conversion,
+// half of a packed multiply-add, one exponential and half of two packed additions; the rank is counted in packed 16-bit numbers.
+// The block maxima stay in shared memory.  The top_k-th largest of 32 maxima over all of them is no larger than the row's top_k-th
+// largest logit, so that only blocks that reach it - few more than top_k - are read a second time (from L2) for the alternatives: every
+// warp keeps a sorted list across its lanes, (value, lowest index) as one 64-bit number, and a list entry's place in the row is its
+// place in its list plus the numbers of larger ones in the other lists.
+// Everything is added in an order that depends on sizes only.  A row whose maximum lies beyond +-2^100 (a mask of the type's lowest
+// value over all of it) or, in y, beyond +-2^20 (a temperature next to zero) is summed again, value by value, against its maximum.
+//
+// Bound: HBM in principle (every logit once); for 16-bit logits the exponentials, 16 per clock and SM, take longer.
+#include <cfloat>
 #include <cmath>
+#include <cooperative_groups.h>
 #include <cstdint>
 
-#include "common.cuh"
+#include "tc_common.cuh"
 
 namespace gb200 {
 
 namespace {
 
-constexpr int kLpThreads = 256;
-constexpr int kLpMaxTop = 32;
+namespace cg = cooperative_groups;
+
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
+constexpr int kLpMaxTop = 32, kLpMaxParts = 8;
+constexpr int kLpVecs = 2, kLpBlockBytes = kLpVecs * 32 * 16;
+constexpr int kLpEntries = 128;   // block maxima that a warp keeps; more blocks share them
+constexpr float kLpHuge = 1.2676506002282294e30f;   // 2^100
+constexpr float kLpFar = 1048576.f;                 // 2^20: the reference, an fp32 number, is then within 2^-4 of the y that it stands for
 
 struct LogProbs {
     const void* logits;
@@ -26,13 +44,118 @@ struct LogProbs {
     float* entropy;
     float* top_log_probs;
     int* top_ids;
-    int vocab, top_k;
+    int vocab, top_k, parts;
     float scale;   // 1 / temperature
 };
 
-__device__ __forceinline__ float lp_value(const float* x, size_t i) { return x[i]; }
-__device__ __forceinline__ float lp_value(const __nv_bfloat16* x, size_t i) { return __bfloat162float(x[i]); }
-__device__ __forceinline__ float lp_value(const __half* x, size_t i) { return __half2float(x[i]); }
+// Sixteen bytes of logits: packed maxima, and their values.
+template <typename T>
+struct LpVec;
+template <>
+struct LpVec<float> {
+    static constexpr int n = 4;
+    __device__ static float top(const uint4& v) { return max_nan(max_nan(__uint_as_float(v.x), __uint_as_float(v.y)), max_nan(__uint_as_float(v.z), __uint_as_float(v.w))); }
+    __device__ static float max_nan(float a, float b)
+    {
+        float r;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+        return r;
+    }
+    __device__ static void values(const uint4& v, float (&x)[4]) { x[0] = __uint_as_float(v.x), x[1] = __uint_as_float(v.y), x[2] = __uint_as_float(v.z), x[3] = __uint_as_float(v.w); }
+    // values with -inf and what lies below -2^100 as -2^100
+    __device__ static void finite(const uint4& v, float (&x)[4])
+    {
+        values(v, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = fmaxf(x[i], -kLpHuge);
+    }
+    struct Count {
+        int n = 0;
+        float than;
+        __device__ explicit Count(float t) : than(t) {}
+        __device__ void add(const uint4& v)
+        {
+            float x[4];
+            values(v, x);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) n += x[i] > than;
+        }
+        __device__ void settle() {}
+    };
+};
+template <typename T2>
+struct LpPairs {
+    static constexpr int n = 8;
+    __device__ static T2 pair(uint32_t w) { return *reinterpret_cast<const T2*>(&w); }
+    __device__ static uint32_t word(T2 p) { return *reinterpret_cast<const uint32_t*>(&p); }
+    __device__ static float low(T2 p);
+    __device__ static float high(T2 p);
+    __device__ static T2 same(float x);
+    __device__ static float top(const uint4& v)
+    {
+        const T2 m = __hmax2_nan(__hmax2_nan(pair(v.x), pair(v.y)), __hmax2_nan(pair(v.z), pair(v.w)));
+        const float a = low(m), b = high(m);
+        return LpVec<float>::max_nan(a, b);
+    }
+    __device__ static void values(const uint4& v, float (&x)[8])
+    {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = low(pair(w[i])), x[2 * i + 1] = high(pair(w[i]));
+    }
+    // values with -inf and what lies below -2^100 as -2^100
+    __device__ static void finite(const uint4& v, float (&x)[8]);
+    // counted as 16-bit floating-point numbers: exact up to 256, and a block adds at most 8 to either half
+    struct Count {
+        int n = 0;
+        T2 than, halves;
+        __device__ explicit Count(float t) : than(same(t)), halves(same(0.f)) {}
+        __device__ void add(const uint4& v)
+        {
+            halves = __hadd2(halves, __hadd2(__hadd2(__hgt2(pair(v.x), than), __hgt2(pair(v.y), than)), __hadd2(__hgt2(pair(v.z), than), __hgt2(pair(v.w), than))));
+        }
+        __device__ void settle()
+        {
+            n += int(low(halves)) + int(high(halves));
+            halves = same(0.f);
+        }
+    };
+};
+template <> __device__ __forceinline__ float LpPairs<__nv_bfloat162>::low(__nv_bfloat162 p) { return __uint_as_float(word(p) << 16); }
+template <> __device__ __forceinline__ float LpPairs<__nv_bfloat162>::high(__nv_bfloat162 p) { return __uint_as_float(word(p) & 0xffff0000u); }
+template <> __device__ __forceinline__ __nv_bfloat162 LpPairs<__nv_bfloat162>::same(float x) { return __float2bfloat162_rn(x); }
+template <> __device__ __forceinline__ float LpPairs<__half2>::low(__half2 p) { return __low2float(p); }
+template <> __device__ __forceinline__ float LpPairs<__half2>::high(__half2 p) { return __high2float(p); }
+template <> __device__ __forceinline__ __half2 LpPairs<__half2>::same(float x) { return __float2half2_rn(x); }
+template <>
+__device__ __forceinline__ void LpPairs<__nv_bfloat162>::finite(const uint4& v, float (&x)[8])
+{
+    const __nv_bfloat162 least = same(-kLpHuge);
+    values(make_uint4(word(__hmax2(pair(v.x), least)), word(__hmax2(pair(v.y), least)), word(__hmax2(pair(v.z), least)), word(__hmax2(pair(v.w), least))), x);
+}
+template <>
+__device__ __forceinline__ void LpPairs<__half2>::finite(const uint4& v, float (&x)[8])   // fp16 has no -2^100
+{
+    values(v, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], -kLpHuge);
+}
+template <>
+struct LpVec<__nv_bfloat16> : LpPairs<__nv_bfloat162> {};
+template <>
+struct LpVec<__half> : LpPairs<__half2> {};
+
+__device__ __forceinline__ float lp_value(const float* x, long long i) { return x[i]; }
+__device__ __forceinline__ float lp_value(const __nv_bfloat16* x, long long i) { return __bfloat162float(x[i]); }
+__device__ __forceinline__ float lp_value(const __half* x, long long i) { return __half2float(x[i]); }
+__device__ __forceinline__ uint32_t lp_bits(const float* x, long long i) { return __float_as_uint(x[i]); }
+__device__ __forceinline__ uint32_t lp_bits(const __nv_bfloat16* x, long long i) { return reinterpret_cast<const uint16_t*>(x)[i]; }
+__device__ __forceinline__ uint32_t lp_bits(const __half* x, long long i) { return reinterpret_cast<const uint16_t*>(x)[i]; }
+
+// -inf
+__device__ __forceinline__ uint32_t lp_none(const float*) { return 0xff800000u; }
+__device__ __forceinline__ uint32_t lp_none(const __nv_bfloat16*) { return 0xff80u; }
+__device__ __forceinline__ uint32_t lp_none(const __half*) { return 0xfc00u; }
 
 // Larger for larger values, the same for +0 and -0; 0 for NaN.
 __device__ __forceinline__ uint32_t lp_key(float x)
@@ -43,75 +166,314 @@ __device__ __forceinline__ uint32_t lp_key(float x)
 }
 __device__ __forceinline__ float lp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-template <typename V, typename Op>
-__device__ __forceinline__ V lp_reduce(V v, Op op)
+// The values of a part of a row: S and W against `ref`, the largest value, how many are above the target, and whether there is a NaN.
+struct LpSum {
+    float ref, s, w, top;
+    int above, nan;
+};
+__device__ __forceinline__ LpSum lp_join(const LpSum& a, const LpSum& b)
 {
-    __shared__ V part[kLpThreads / 32];
-    __shared__ V all;
+    LpSum r;
+    r.ref = fmaxf(a.ref, b.ref);
+    const float da = a.ref - r.ref, db = b.ref - r.ref, fa = ex2(da), fb = ex2(db);
+    r.s = fa * a.s + fb * b.s;
+    r.w = (fa > 0.f ? fa * (a.w + da * a.s) : 0.f) + (fb > 0.f ? fb * (b.w + db * b.s) : 0.f);
+    r.top = fmaxf(a.top, b.top);
+    r.above = a.above + b.above, r.nan = a.nan | b.nan;
+    return r;
+}
+
+// A part's results in shared memory, read by the others of its cluster.
+struct LpPart {
+    LpSum sum;
+    unsigned long long top[kLpMaxTop];
+};
+struct LpShared {
+    LpPart part;
+    LpSum sums[kLpWarps];
+    unsigned long long lists[kLpWarps][kLpMaxTop];
+    float maxima[kLpEntries * kLpWarps];   // [entry][warp]
+};
+
+// The entries of `count` lists of 32 in descending order (0: none), one per thread, to their places among the first `most` of all of them.
+template <typename Lists>
+__device__ __forceinline__ void lp_merge(const Lists& lists, int count, int most, unsigned long long* out)
+{
+    const int mine = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (mine >= count) return;
+    const unsigned long long key = lists(mine)[lane];
+    int place = lane;
+    for (int l = 0; l < count; ++l) {
+        if (l == mine) continue;
+        const unsigned long long* list = lists(l);
+        int larger = 0;   // how many of the list are larger: 0 .. 32
 #pragma unroll
-    for (int o = 16; o; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kLpThreads / 32; ++w) v = op(v, part[w]);
-        all = v;
+        for (int step = 16; step; step >>= 1)
+            if (list[larger + step - 1] > key) larger += step;
+        if (larger == 31 && list[31] > key) larger = 32;
+        place += larger;
     }
-    __syncthreads();
-    return all;
+    if (key && place < most) out[place] = key;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLpThreads) log_probs_kernel(const LogProbs p)
+__global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs p)
 {
+    using Vec = LpVec<T>;
+    constexpr int kBlock = kLpBlockBytes / int(sizeof(T));
+    __shared__ LpShared sh;
     pdl_launch_dependents();
     pdl_wait();
-    const size_t r = blockIdx.x;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = int(blockIdx.x) % p.parts;
+    const size_t r = blockIdx.x / unsigned(p.parts);
     const T* row = static_cast<const T*>(p.logits) + r * p.stride;
-    const auto larger = [](auto a, auto b) { return a > b ? a : b; };
-    const auto plus = [](auto a, auto b) { return a + b; };
+    // blocks start on 16-byte boundaries: value i of the row is value i + skip of its blocks
+    const int skip = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const T* base = row - skip;
+    const int blocks = int(((long long)p.vocab + skip + kBlock - 1) / kBlock);
+    const int block0 = int((long long)part * blocks / p.parts), block1 = int((long long)(part + 1) * blocks / p.parts);
     const int target = p.targets ? p.targets[r] : -1;
     const bool given = target >= 0 && target < p.vocab;
-    const float x_t = given ? lp_value(row, target) : 0.f;
-    float top = -INFINITY;
-    for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) top = fmaxf(top, lp_value(row, i));
-    top = lp_reduce(top, larger);
-    const bool empty = top == -INFINITY;   // a row of -inf (or of -inf and NaN)
-    float sum = 0.f, weighted = 0.f;
-    int above = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
-        const float x = lp_value(row, i);
-        above += x > x_t;
-        const float d = x == -INFINITY ? -INFINITY : (x - top) * p.scale, e = expf(d);
-        sum += e;
-        weighted += d == -INFINITY ? 0.f : e * d;
+    const float x_t = given ? lp_value(row, target) : INFINITY;
+    const float scale = p.scale * 1.4426950408889634f;
+
+    // a lane's vectors of a block; what lies outside the row is -inf
+    const auto load = [&](int b, uint4 (&v)[kLpVecs]) {
+        const long long first = (long long)b * kBlock - skip;
+        const uint4* from = reinterpret_cast<const uint4*>(base + (long long)b * kBlock) + lane;
+        if (first >= 0 && first + kBlock <= p.vocab) {
+#pragma unroll
+            for (int k = 0; k < kLpVecs; ++k) v[k] = __ldg(from + 32 * k);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kLpVecs; ++k) {
+                const long long at = first + (k * 32 + lane) * Vec::n;
+                uint32_t w[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    constexpr int per = Vec::n / 4;
+                    const uint32_t none = lp_none(row);
+                    uint32_t bits = 0;
+#pragma unroll
+                    for (int h = 0; h < per; ++h) {
+                        const long long e = at + i * per + h;
+                        bits |= (e >= 0 && e < p.vocab ? lp_bits(row, e) : none) << (16 * h);
+                    }
+                    w[i] = bits;
+                }
+                v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        }
+    };
+
+    const int rounds = (block1 - block0 + kLpWarps - 1) / kLpWarps;          // blocks of a warp
+    const int shared_by = (rounds + kLpEntries - 1) / kLpEntries, entries = (rounds + shared_by - 1) / shared_by;
+    float ref = -kLpHuge * scale, entry = -INFINITY, top = -INFINITY;       // ref: in powers of two
+    int nan = 0;
+    uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
+    typename Vec::Count count(x_t);
+    const uint64_t scale2 = f32x2(scale, scale);
+    uint4 v[kLpVecs], ahead[kLpVecs];
+    if (block0 + warp < block1) load(block0 + warp, ahead);
+    for (int i = 0; i < rounds; ++i) {
+        const int b = block0 + i * kLpWarps + warp;
+        float m = -INFINITY;
+        if (b < block1) {
+#pragma unroll
+            for (int k = 0; k < kLpVecs; ++k) v[k] = ahead[k];
+            if (b + kLpWarps < block1) load(b + kLpWarps, ahead);
+            m = LpVec<float>::max_nan(Vec::top(v[0]), Vec::top(v[1]));
+            asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+            const float y = m * scale;
+            if (!(y <= ref + 8.f)) {
+                if (isnan(m)) {
+                    nan = 1;
+                } else if (m <= kLpHuge) {   // beyond that the row is summed again
+                    const float d = ref - y, f = ex2(d);
+                    const uint64_t f2 = f32x2(f, f), d2 = f32x2(fmaxf(d, -1e30f), fmaxf(d, -1e30f));
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        w2[k] = mul2(f2, fma2(d2, s2[k], w2[k]));
+                        s2[k] = mul2(f2, s2[k]);
+                    }
+                    ref = y;
+                }
+            }
+            const uint64_t minus2 = f32x2(-ref, -ref);
+#pragma unroll
+            for (int k = 0; k < kLpVecs; ++k) {
+                float x[Vec::n];
+                Vec::finite(v[k], x);
+                count.add(v[k]);
+#pragma unroll
+                for (int e = 0; e < Vec::n; e += 2) {
+                    const uint64_t d = fma2(f32x2(x[e], x[e + 1]), scale2, minus2);
+                    float a, c;
+                    f32x2_split(d, a, c);
+                    const uint64_t p2 = f32x2(ex2(a), ex2(c));
+                    s2[(e >> 1) & 1] = add2(s2[(e >> 1) & 1], p2);
+                    w2[(e >> 1) & 1] = fma2(p2, d, w2[(e >> 1) & 1]);
+                }
+            }
+            if ((i & 31) == 31) count.settle();
+        }
+        // a block with a NaN counts as one that may hold alternatives, and not for the bound on them
+        if (isnan(m)) entry = m;
+        else if (!isnan(entry)) entry = fmaxf(entry, m);
+        top = fmaxf(top, m);
+        if ((i + 1) % shared_by == 0 || i + 1 == rounds) {
+            if (lane == 0) sh.maxima[i / shared_by * kLpWarps + warp] = entry;
+            entry = -INFINITY;
+        }
     }
-    sum = lp_reduce(sum, plus);
-    weighted = lp_reduce(weighted, plus);
-    above = lp_reduce(above, plus);
-    const float log_sum = logf(sum);
-    const auto log_prob = [&](float x) { return isnan(sum) ? sum : empty || x == -INFINITY ? -INFINITY : (x - top) * p.scale - log_sum; };
+    count.settle();
+    {
+        LpSum mine;
+        float a, b, c, d;
+        f32x2_split(add2(s2[0], s2[1]), a, b);
+        f32x2_split(add2(w2[0], w2[1]), c, d);
+        mine.s = a + b, mine.w = c + d;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            mine.s += __shfl_xor_sync(0xffffffffu, mine.s, o);
+            mine.w += __shfl_xor_sync(0xffffffffu, mine.w, o);
+        }
+        mine.ref = ref, mine.top = top, mine.nan = nan;
+        mine.above = __reduce_add_sync(0xffffffffu, count.n);
+        if (lane == 0) sh.sums[warp] = mine;
+    }
+    __syncthreads();
+
+    // ---- alternatives of the part: a list per warp, merged
+    if (p.top_k) {
+        // the top_k-th largest of the lanes' maxima over all blocks: at least top_k values are as large
+        float bound = -INFINITY;
+        for (int i = lane; i < entries * kLpWarps; i += 32) bound = fmaxf(bound, sh.maxima[i]);   // a NaN loses
+        uint32_t key = lp_key(bound);
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (int d = size >> 1; d; d >>= 1) {   // bitonic, descending
+                const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
+                const bool keep_large = ((lane & size) == 0) == ((lane & d) == 0);
+                key = keep_large ? max(key, o) : min(key, o);
+            }
+        bound = lp_unkey(__shfl_sync(0xffffffffu, key, p.top_k - 1));
+        unsigned long long list = 0, least = 0;   // the lane's entry; the top_k-th
+        for (int e = 0; e < entries; ++e) {
+            const float m = sh.maxima[e * kLpWarps + warp];
+            if (m < bound) continue;   // not for NaN
+            for (int i = e * shared_by; i < min(rounds, (e + 1) * shared_by); ++i) {
+                const int b = block0 + i * kLpWarps + warp;
+                if (b >= block1) break;
+                load(b, v);
+#pragma unroll
+                for (int k = 0; k < kLpVecs; ++k) {
+                    if (!__any_sync(0xffffffffu, !(Vec::top(v[k]) < bound))) continue;
+                    float x[Vec::n];
+                    Vec::values(v[k], x);
+#pragma unroll 1
+                    for (int n = 0; n < Vec::n; ++n) {
+                        float mine = x[0];
+#pragma unroll
+                        for (int t = 1; t < Vec::n; ++t) mine = n == t ? x[t] : mine;
+                        const long long at = (long long)b * kBlock - skip + (k * 32 + lane) * Vec::n + n;
+                        const unsigned long long c = mine >= bound && at >= 0 && at < p.vocab ? ((unsigned long long)lp_key(mine) << 32) | (0xffffffffu - uint32_t(at)) : 0;
+                        for (uint32_t todo = __ballot_sync(0xffffffffu, c > least); todo; todo &= todo - 1) {
+                            const unsigned long long in = __shfl_sync(0xffffffffu, c, __ffs(todo) - 1);
+                            if (in <= least) continue;
+                            const int place = __popc(__ballot_sync(0xffffffffu, list > in));
+                            const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
+                            list = lane < place ? list : lane == place ? in : before;
+                            least = __shfl_sync(0xffffffffu, list, p.top_k - 1);
+                        }
+                    }
+                }
+            }
+        }
+        sh.lists[warp][lane] = list;
+        if (warp == 0) sh.part.top[lane] = 0;
+        __syncthreads();
+        lp_merge([&](int l) { return sh.lists[l]; }, kLpWarps, p.top_k, sh.part.top);
+    }
     if (threadIdx.x == 0) {
-        if (p.targets) {
-            p.log_probs[r] = given ? log_prob(x_t) : 0.f;
-            p.ranks[r] = given ? above + 1 : 0;
-        }
-        if (p.entropy) p.entropy[r] = isnan(sum) ? sum : empty ? 0.f : log_sum - weighted / sum;
+        LpSum all = sh.sums[0];
+        for (int w = 1; w < kLpWarps; ++w) all = lp_join(all, sh.sums[w]);
+        sh.part.sum = all;
     }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < p.top_k; ++k) {
-        unsigned long long best = 0;
-        for (int i = threadIdx.x; i < p.vocab; i += kLpThreads) {
-            const uint32_t key = lp_key(lp_value(row, i));
-            const unsigned long long c = (static_cast<unsigned long long>(key) << 32) | (0xffffffffu - uint32_t(i));
-            if (key && c < last && c > best) best = c;
+
+    // ---- the parts of the row
+    cg::cluster_group cluster = cg::this_cluster();
+    if (p.parts > 1) cluster.sync();
+    else __syncthreads();
+    const auto part_of = [&](int c) -> const LpPart& { return p.parts > 1 ? *cluster.map_shared_rank(&sh.part, c) : sh.part; };
+    LpSum all = part_of(0).sum;
+    for (int c = 1; c < p.parts; ++c) all = lp_join(all, part_of(c).sum);
+    const bool empty = all.top == -INFINITY && !all.nan;   // a row of -inf
+    const bool huge = !all.nan && !empty && !(fabsf(all.top) <= kLpHuge && fabsf(all.top) * scale <= kLpFar);
+    if (huge) {
+        // summed again against the maximum, value by value
+        if (p.parts > 1) cluster.sync();   // the others have read this part's sums
+        else __syncthreads();
+        float s = 0.f, w = 0.f;
+        const long long from = max(0ll, (long long)block0 * kBlock - skip), to = min((long long)p.vocab, (long long)block1 * kBlock - skip);
+        for (long long i = from + threadIdx.x; i < to; i += kLpThreads) {
+            const float d = (lp_value(row, i) - all.top) * scale, e = ex2(d);
+            s += e;
+            w += e > 0.f ? e * d : 0.f;   // inf - inf is NaN, and s with it
         }
-        best = lp_reduce(best, larger);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            w += __shfl_xor_sync(0xffffffffu, w, o);
+        }
+        if (lane == 0) sh.sums[warp].s = s, sh.sums[warp].w = w;
+        __syncthreads();
         if (threadIdx.x == 0) {
-            p.top_ids[r * p.top_k + k] = best ? int(0xffffffffu - uint32_t(best)) : -1;
-            p.top_log_probs[r * p.top_k + k] = best ? log_prob(lp_unkey(uint32_t(best >> 32))) : NAN;
+            for (int k = 1; k < kLpWarps; ++k) s += sh.sums[k].s, w += sh.sums[k].w;
+            sh.part.sum.s = s, sh.part.sum.w = w;
         }
-        last = best;
+        if (p.parts > 1) cluster.sync();
+        else __syncthreads();
+        all.s = part_of(0).sum.s, all.w = part_of(0).sum.w;
+        for (int c = 1; c < p.parts; ++c) all.s += part_of(c).sum.s, all.w += part_of(c).sum.w;
     }
+    if (part == 0) {
+        const float log2_s = log2f(all.s);
+        constexpr float kLn2 = 0.6931471805599453f;
+        const auto log_prob = [&](float x) -> float {
+            if (all.nan || isnan(all.s)) return NAN;
+            if (empty || x == -INFINITY) return -INFINITY;
+            // rounding may leave a sole value's a little above 0
+            if (huge || x < -kLpHuge) return fminf(0.f, (x - all.top) * p.scale - log2_s * kLn2);
+            return fminf(0.f, (fmaf(x, scale, -all.ref) - log2_s) * kLn2);
+        };
+        if (threadIdx.x == 0) {
+            if (p.targets) {
+                p.log_probs[r] = given ? log_prob(x_t) : 0.f;
+                p.ranks[r] = given ? all.above + 1 : 0;
+            }
+            if (p.entropy) p.entropy[r] = all.nan || isnan(all.s) ? NAN : empty ? 0.f : fmaxf(0.f, (log2_s - all.w / all.s) * kLn2);
+        }
+        if (p.top_k) {
+            // sh.lists is free: every warp of this CTA has come through the barrier above
+            const unsigned long long* result = sh.part.top;
+            if (p.parts > 1) {
+                if (threadIdx.x < kLpMaxTop) sh.lists[0][threadIdx.x] = 0;
+                __syncthreads();
+                lp_merge([&](int l) { return part_of(l).top; }, p.parts, p.top_k, sh.lists[0]);
+                __syncthreads();
+                result = sh.lists[0];
+            }
+            if (int(threadIdx.x) < p.top_k) {
+                const unsigned long long key = result[threadIdx.x];
+                p.top_ids[r * p.top_k + threadIdx.x] = key ? int(0xffffffffu - uint32_t(key)) : -1;
+                p.top_log_probs[r * p.top_k + threadIdx.x] = key ? log_prob(lp_unkey(uint32_t(key >> 32))) : NAN;
+            }
+        }
+    }
+    if (p.parts > 1) cluster.sync();   // the first part may still read this one
 }
 
 }  // namespace
@@ -131,23 +493,30 @@ int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, c
         return fail(GARNET_B200_INVALID_VALUE, "log_probs: unknown dtype %d", dtype);
     if (reinterpret_cast<uintptr_t>(d_logits) & (dtype == GARNET_B200_FP32 ? 3 : 1))
         return fail(GARNET_B200_INVALID_VALUE, "log_probs: the logits are not aligned to their values");
-    if (!(temperature > 0.f) || !std::isfinite(temperature) || !std::isfinite(1.f / temperature))
-        return fail(GARNET_B200_INVALID_VALUE, "log_probs: the temperature must be positive and finite");
+    if (!(temperature >= 1e-6f && temperature <= 1e6f))
+        return fail(GARNET_B200_INVALID_VALUE, "log_probs: the temperature must lie between 1e-6 and 1e6");
     if (!d_targets != !d_log_probs || !d_targets != !d_ranks)
         return fail(GARNET_B200_INVALID_VALUE, "log_probs: targets, log_probs and ranks are given together");
     if (top_k < 0 || top_k > vocab || (top_k > 0 && (!d_top_log_probs || !d_top_ids)))
         return fail(GARNET_B200_INVALID_VALUE, "log_probs: bad top_k %d, or no arrays for it", top_k);
     if (top_k > kLpMaxTop) return fail(GARNET_B200_NOT_SUPPORTED, "log_probs: top_k above %d", kLpMaxTop);
-    const LogProbs p{d_logits, row_stride, d_targets, d_log_probs, d_ranks, d_entropy, d_top_log_probs, d_top_ids, vocab, top_k, 1.f / temperature};
+    // as many parts as run at once, four CTAs to an SM, each with a block for every warp
+    const long long blocks = (long long)vocab * (dtype == GARNET_B200_FP32 ? 4 : 2) / kLpBlockBytes;
+    int parts = 1;
+    while (parts < kLpMaxParts && (long long)rows * parts * 2 <= 4 * kSmCount && blocks >= 2 * parts * kLpWarps) parts *= 2;
+    if ((long long)rows * parts > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "log_probs: too many rows");
+    const LogProbs p{d_logits, row_stride, d_targets, d_log_probs, d_ranks, d_entropy, d_top_log_probs, d_top_ids, vocab, top_k, parts, 1.f / temperature};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(rows));
+    cfg.gridDim = dim3(unsigned(rows) * unsigned(parts));
     cfg.blockDim = dim3(kLpThreads);
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {unsigned(parts), 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = (flags & 1u) ? 1 : 0;
+    cfg.numAttrs = (flags & 1u) ? 2 : 1;
     GB_CUDA(cudaLaunchKernelEx(&cfg, dtype == GARNET_B200_BF16 ? log_probs_kernel<__nv_bfloat16> : dtype == GARNET_B200_FP16 ? log_probs_kernel<__half> : log_probs_kernel<float>, p));
     return GARNET_B200_OK;
 }

@@ -355,7 +355,7 @@ int garnet_b200_embedding_gather(const void* d_table, const int* d_ids, void* d_
 int garnet_b200_argmax_bf16(const void* d_logits, int* d_out, int batch, int vocab, unsigned flags, void* stream);
 
 /* Log probabilities of rows of logits z [rows, vocab] (dtype GARNET_B200_BF16, _FP16 or _FP32, rows `row_stride` elements apart)
- * under p = softmax(z / temperature):
+ * under p = softmax(z / temperature), temperature between 1e-6 and 1e6:
  *   d_log_probs[r]  log p(d_targets[r])        d_ranks[r]  1 + how many logits are larger than the target's
  *   d_entropy[r]    -sum p log p               d_top_ids / d_top_log_probs [rows, top_k]: the largest logits in descending order,
  *                                              the lowest index first among equals

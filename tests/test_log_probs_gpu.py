@@ -32,6 +32,7 @@ def oracle(x, targets, k, temperature):
         entropy = np.where(empty, 0.0, -(p * np.where(e > 0, lp, 0.0)).sum(1))
         mean_d, mean_d2 = (p * ad).sum(1), (p * ad * ad).sum(1)
     lp[empty] = -np.inf
+    lp[lp < -np.finfo(np.float32).max] = -np.inf     # beyond fp32
     n = x.shape[1]
     tol_s = U * (3 * mean_d + n / 256 + 20)
     tol_h = tol_s + U * (mean_d * (n / 256 + 24) + 3 * mean_d2)
@@ -98,22 +99,27 @@ def test_orders_and_ties(dtype, rows):
         check(x, targets, 32)
 
 
-@pytest.mark.parametrize("rows_each", [1, 60])
-def test_masked_rows(rows_each):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows_each,temperature", [(1, 1.0), (60, 1.0), (1, 60000.0), (1, 2e-6)])
+def test_masked_rows(dtype, rows_each, temperature):
     """-inf and the type's lowest value as masks, masks that leave one value or none, rows without a target."""
-    n, inf = 3001, float("inf")
+    n, inf, lowest = 3001, float("inf"), torch.finfo(dtype).min
     gen = torch.Generator(device="cuda").manual_seed(9)
-    x = torch.randn(6, n, device="cuda", generator=gen)
+    x = torch.randn(9, n, device="cuda", generator=gen)
     x[0, ::2] = -inf
     x[1] = -inf
     x[2] = -inf
     x[2, 1777] = -3.0
-    x[3, 5:] = torch.finfo(torch.bfloat16).min
-    x[4] = torch.finfo(torch.bfloat16).min
+    x[3, 5:] = lowest
+    x[4] = lowest
     x[5, :2990] = -inf
-    x = x.to(torch.bfloat16).repeat(rows_each, 1)
-    targets = torch.tensor([0, 3, 1777, 7, -1, n], dtype=torch.int32, device="cuda").repeat(rows_each)
-    r = check(x, targets, 32)
+    x[6] = lowest                       # one mask over the other
+    x[6, 100:2900] = -inf
+    x[7] = -lowest
+    x[8, :2000], x[8, 2000:] = lowest, -lowest
+    x = x.to(dtype).repeat(rows_each, 1)
+    targets = torch.tensor([0, 3, 1777, 7, -1, n, 5, 6, 2999], dtype=torch.int32, device="cuda").repeat(rows_each)
+    r = check(x, targets, 32, temperature)
     assert r.entropy[1] == 0 and r.log_probs[1] == -inf and r.log_probs[2] == 0 and r.log_probs[4] == 0 and r.ranks[4] == 0 and r.ranks[5] == 0
 
 
