@@ -159,13 +159,16 @@ def stream_ptr() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
-def on_device(t, name: str, dtype=None, shape=None):
+def on_device(t, name: str, dtype, shape):
     """`t` when it is a contiguous CUDA tensor on the current device, of the given type and shape (None in a shape: any extent)."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() >= 0
+            and t.get_device() == torch._C._cuda_getDevice()):
+        return t
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device.index != torch.cuda.current_device():
         raise ValueError(f"{name} must be a tensor on the current CUDA device")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, not {t.dtype}")
-    if shape is not None and (t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape))):
+    if t.dim() != len(shape) or any(w is not None and w != n for w, n in zip(shape, t.shape)):
         raise ValueError(f"{name} must have the shape {tuple('any' if w is None else w for w in shape)}, not {tuple(t.shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")

@@ -29,7 +29,7 @@ class PagePool:
         if len(shape) < 3:
             raise ValueError("the pages of a layer must be [pages, page_size, ...]")
         for i, t in enumerate(keys + values):
-            on_device(t, f"the pages of layer {i % len(keys)}", keys[0].dtype, shape)
+            on_device(t, f"the pages of layer {i % len(keys)}", keys[0].dtype, tuple(shape))
         self._keep = keys, values
         self.device = keys[0].device
         self.opt = CacheOptions(abi=1, struct_size=ctypes.sizeof(CacheOptions), layers=len(keys), physical_pages=shape[0], page_size=shape[1],
@@ -42,18 +42,22 @@ class PagePool:
         self.page_tables = torch.full((sequences, max_logical_pages), -1, dtype=torch.int32, device=self.device)
         self.lengths = torch.zeros(sequences, dtype=torch.int32, device=self.device)
         self.refcounts = torch.zeros(shape[0], dtype=torch.int32, device=self.device)
+        # what every call passes, at hand
+        self._opt = ctypes.byref(self.opt)
+        self._state = self.page_tables.data_ptr(), self.lengths.data_ptr(), self.refcounts.data_ptr()
+        self._work = self._ws.data_ptr(), need.value
 
-    def _list(self, t, name: str, count=None):
+    def _list(self, t, name: str, count: int):
         on_device(t, name, torch.int32, (count,))
-        if t.device != self.device:
+        if t.get_device() != self.device.index:
             raise ValueError(f"{name} is on another device than the pool")
-        return t
+        return count
 
-    def _entries(self, t, name: str):
-        self._list(t, name)
-        if t.numel() > self.opt.sequences:
+    def _entries(self, t, name: str) -> int:
+        n = self._list(t, name, t.numel())
+        if n > self.opt.sequences:
             raise ValueError(f"{name} has more entries than the pool has sequences")
-        return t.numel()
+        return n
 
     def extend(self, sequences, tokens):
         """sequences[i] grows by tokens[i] positions.  Returns a status per entry (0; 1: refused; 5: too few free pages)."""
@@ -61,9 +65,8 @@ class PagePool:
         self._list(tokens, "tokens", n)
         status = torch.empty(n, dtype=torch.int32, device=self.device)
         if n:
-            check(lib().garnet_b200_cache_extend(ctypes.byref(self.opt), self.page_tables.data_ptr(), self.lengths.data_ptr(),
-                                                 self.refcounts.data_ptr(), sequences.data_ptr(), tokens.data_ptr(), status.data_ptr(), n,
-                                                 self._ws.data_ptr(), self._ws.numel(), stream_ptr()))
+            check(lib().garnet_b200_cache_extend(self._opt, *self._state, sequences.data_ptr(), tokens.data_ptr(), status.data_ptr(), n,
+                                                 *self._work, stream_ptr()))
         return status
 
     def fork(self, parents, children):
@@ -72,30 +75,28 @@ class PagePool:
         self._list(children, "children", n)
         status = torch.empty(n, dtype=torch.int32, device=self.device)
         if n:
-            check(lib().garnet_b200_cache_fork(ctypes.byref(self.opt), self._k, self._v, self.page_tables.data_ptr(), self.lengths.data_ptr(),
-                                               self.refcounts.data_ptr(), parents.data_ptr(), children.data_ptr(), status.data_ptr(), n,
-                                               self._ws.data_ptr(), self._ws.numel(), stream_ptr()))
+            check(lib().garnet_b200_cache_fork(self._opt, self._k, self._v, *self._state, parents.data_ptr(), children.data_ptr(),
+                                               status.data_ptr(), n, *self._work, stream_ptr()))
         return status
 
     def free(self, sequences) -> None:
         """The sequences give their pages back and are empty."""
         n = self._entries(sequences, "sequences")
         if n:
-            check(lib().garnet_b200_cache_free(ctypes.byref(self.opt), self.page_tables.data_ptr(), self.lengths.data_ptr(),
-                                               self.refcounts.data_ptr(), sequences.data_ptr(), n, stream_ptr()))
+            check(lib().garnet_b200_cache_free(self._opt, *self._state, sequences.data_ptr(), n, stream_ptr()))
 
     def compact(self):
         """Moves the live pages to the numbers 0 .. live - 1.  Returns live, a device tensor of one number."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         if torch.cuda.current_device() != self.device.index:
             raise ValueError("the pool is on another device than the current one")
-        check(lib().garnet_b200_cache_compact(ctypes.byref(self.opt), self._k, self._v, self.page_tables.data_ptr(),
-                                              self.refcounts.data_ptr(), live.data_ptr(), self._ws.data_ptr(), self._ws.numel(), stream_ptr()))
+        check(lib().garnet_b200_cache_compact(self._opt, self._k, self._v, self._state[0], self._state[2], live.data_ptr(), *self._work,
+                                              stream_ptr()))
         return live
 
     def copy_pages(self, src, dst) -> None:
         """Page dst[i] becomes a copy of page src[i] in every layer, as if one pair after the other."""
-        n = self._list(src, "src").numel()
+        n = self._list(src, "src", src.numel())
         self._list(dst, "dst", n)
         if n:
-            check(lib().garnet_b200_cache_copy_pages(ctypes.byref(self.opt), self._k, self._v, src.data_ptr(), dst.data_ptr(), n, stream_ptr()))
+            check(lib().garnet_b200_cache_copy_pages(self._opt, self._k, self._v, src.data_ptr(), dst.data_ptr(), n, stream_ptr()))

@@ -7,10 +7,10 @@
 // turn: two 16-byte loads per lane, the block's maximum (NaN wins) by packed maxima and one warp reduction, which also says whether the
 // warp's reference has to grow (by more than 2^8, so that this is rare: S and W are rescaled then), then per value one conversion,
 // half of a packed multiply-add, one exponential and half of two packed additions; the rank is counted in packed 16-bit numbers.
-// The block maxima stay in shared memory.  The top_k-th largest of 32 maxima over all of them is no larger than the row's top_k-th
-// largest logit, so that only blocks that reach it - few more than top_k - are read a second time (from L2) for the alternatives: every
-// warp keeps a sorted list across its lanes, (value, lowest index) as one 64-bit number, and a list entry's place in the row is its
-// place in its list plus the numbers of larger ones in the other lists.
+// The block maxima stay in shared memory.  With n warps the ceil(top_k / n)-th largest of a warp's 32 lane maxima, of all warps the least, is
+// no larger than the top_k-th largest logit, so that only blocks that reach it are read a second time (from L2) for the alternatives: every
+// value that reaches it becomes a candidate, (value, lowest index) as one 64-bit number, and the candidates larger than it say its place.
+// Where too many are equal for that, every warp keeps a sorted list across its lanes.
 // Everything is added in an order that depends on sizes only.  A row whose maximum lies beyond +-2^100 (a mask of the type's lowest
 // value over all of it) or, in y, beyond +-2^20 (a temperature next to zero) is summed again, value by value, against its maximum.
 //
@@ -30,6 +30,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32, kLpMaxParts = 8;
+constexpr int kLpCandidates = 256;
 constexpr int kLpVecs = 2, kLpBlockBytes = kLpVecs * 32 * 16;
 constexpr int kLpEntries = 128;   // block maxima that a warp keeps; more blocks share them
 constexpr float kLpHuge = 1.2676506002282294e30f;   // 2^100
@@ -164,6 +165,8 @@ __device__ __forceinline__ uint32_t lp_key(float x)
     const uint32_t b = __float_as_uint(x + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+// A value and its place: larger values first, then lower places.
+__device__ __forceinline__ unsigned long long lp_entry(float x, long long i) { return (static_cast<unsigned long long>(lp_key(x)) << 32) | (0xffffffffu - uint32_t(i)); }
 __device__ __forceinline__ float lp_unkey(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 // The values of a part of a row: S and W against `ref`, the largest value, how many are above the target, and whether there is a NaN.
@@ -183,7 +186,21 @@ __device__ __forceinline__ LpSum lp_join(const LpSum& a, const LpSum& b)
     return r;
 }
 
-// A part's results in shared memory, read by the others of its cluster.
+// The same over 8 lanes' sums, in a fixed order; every lane of the warp that asks gets the result.
+__device__ __forceinline__ LpSum lp_join_lanes(LpSum v)
+{
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) {
+        LpSum o;
+        o.ref = __shfl_xor_sync(0xffffffffu, v.ref, d), o.s = __shfl_xor_sync(0xffffffffu, v.s, d), o.w = __shfl_xor_sync(0xffffffffu, v.w, d);
+        o.top = __shfl_xor_sync(0xffffffffu, v.top, d);
+        o.above = __shfl_xor_sync(0xffffffffu, v.above, d), o.nan = __shfl_xor_sync(0xffffffffu, v.nan, d);
+        v = (threadIdx.x & d) ? lp_join(o, v) : lp_join(v, o);   // the lower lanes' sum first
+    }
+    return v;
+}
+
+// A part's results in shared memory, read by the first of its cluster.
 struct LpPart {
     LpSum sum;
     unsigned long long top[kLpMaxTop];
@@ -191,28 +208,41 @@ struct LpPart {
 struct LpShared {
     LpPart part;
     LpSum sums[kLpWarps];
-    unsigned long long lists[kLpWarps][kLpMaxTop];
-    float maxima[kLpEntries * kLpWarps];   // [entry][warp]
+    int found;                                        // candidates in `keys`, or more than there is room for
+    unsigned long long keys[kLpCandidates];           // candidates in no order; or lists of 32, one per warp; or the parts' lists
+    unsigned long long out[kLpMaxTop];
+    float bounds[kLpWarps];
+    float maxima[kLpEntries * kLpWarps];              // [entry][warp]
 };
 
-// The entries of `count` lists of 32 in descending order (0: none), one per thread, to their places among the first `most` of all of them.
-template <typename Lists>
-__device__ __forceinline__ void lp_merge(const Lists& lists, int count, int most, unsigned long long* out)
+// The largest `most` of `count` different keys, up to one per thread, to out[0 ..] in descending order; 0 where there are fewer.
+__device__ __forceinline__ void lp_rank(const unsigned long long* keys, int count, int most, unsigned long long* out)
 {
-    const int mine = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (mine >= count) return;
-    const unsigned long long key = lists(mine)[lane];
-    int place = lane;
-    for (int l = 0; l < count; ++l) {
-        if (l == mine) continue;
-        const unsigned long long* list = lists(l);
-        int larger = 0;   // how many of the list are larger: 0 .. 32
+    if (int(threadIdx.x) >= count && int(threadIdx.x) < most) out[threadIdx.x] = 0;
+    if (int(threadIdx.x & ~31u) >= count) return;
+    const unsigned long long key = int(threadIdx.x) < count ? keys[threadIdx.x] : 0;
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) place += keys[i] > key;
+    if (key && place < most) out[place] = key;
+}
+
+// The same of `lists` descending lists of 32, which 0 may follow: a key's place is its place in its list and the numbers of larger keys in
+// the others.  Out's 32 entries are 0 before.
+__device__ __forceinline__ void lp_merge(const unsigned long long* keys, int lists, int most, unsigned long long* out)
+{
+    const int mine = threadIdx.x >> 5;
+    if (mine >= lists) return;
+    const unsigned long long key = keys[threadIdx.x];
+    int larger[kLpWarps] = {};
 #pragma unroll
-        for (int step = 16; step; step >>= 1)
-            if (list[larger + step - 1] > key) larger += step;
-        if (larger == 31 && list[31] > key) larger = 32;
-        place += larger;
-    }
+    for (int step = 16; step; step >>= 1)
+#pragma unroll
+        for (int l = 0; l < kLpWarps; ++l)
+            if (l < lists && keys[l * 32 + larger[l] + step - 1] > key) larger[l] += step;
+    int place = 0;
+#pragma unroll
+    for (int l = 0; l < kLpWarps; ++l) place += l < lists ? larger[l] + (larger[l] == 31 && keys[l * 32 + 31] > key) : 0;
     if (key && place < most) out[place] = key;
 }
 
@@ -233,9 +263,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
     const T* base = row - skip;
     const int blocks = int(((long long)p.vocab + skip + kBlock - 1) / kBlock);
     const int block0 = int((long long)part * blocks / p.parts), block1 = int((long long)(part + 1) * blocks / p.parts);
-    const int target = p.targets ? p.targets[r] : -1;
-    const bool given = target >= 0 && target < p.vocab;
-    const float x_t = given ? lp_value(row, target) : INFINITY;
     const float scale = p.scale * 1.4426950408889634f;
 
     // a lane's vectors of a block; what lies outside the row is -inf
@@ -268,14 +295,25 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
     };
 
     const int rounds = (block1 - block0 + kLpWarps - 1) / kLpWarps;          // blocks of a warp
+    if (rounds > 1 && rounds <= 16) {
+        // a short part: all of it is asked for at once, eight lanes per block of 1 KB
+        for (int i = lane >> 3; i < rounds; i += 4) {
+            const long long at = (long long)(block0 + i * kLpWarps + warp) * kLpBlockBytes + (lane & 7) * 128;
+            if (block0 + i * kLpWarps + warp < block1 && at >= 0 && at < ((long long)p.vocab + skip) * int(sizeof(T)))
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(base) + at));
+        }
+    }
     const int shared_by = (rounds + kLpEntries - 1) / kLpEntries, entries = (rounds + shared_by - 1) / shared_by;
-    float ref = -kLpHuge * scale, entry = -INFINITY, top = -INFINITY;       // ref: in powers of two
+    float ref = -kLpHuge * scale, entry = -INFINITY, top = -INFINITY, lane_top = -INFINITY;   // ref: in powers of two
     int nan = 0;
     uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
-    typename Vec::Count count(x_t);
     const uint64_t scale2 = f32x2(scale, scale);
     uint4 v[kLpVecs], ahead[kLpVecs];
-    if (block0 + warp < block1) load(block0 + warp, ahead);
+    if (block0 + warp < block1) load(block0 + warp, ahead);   // asked for before the two dependent loads of the target's logit
+    const int target = p.targets ? p.targets[r] : -1;
+    const bool given = target >= 0 && target < p.vocab;
+    const float x_t = given ? lp_value(row, target) : INFINITY;
+    typename Vec::Count count(x_t);
     for (int i = 0; i < rounds; ++i) {
         const int b = block0 + i * kLpWarps + warp;
         float m = -INFINITY;
@@ -284,6 +322,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
             for (int k = 0; k < kLpVecs; ++k) v[k] = ahead[k];
             if (b + kLpWarps < block1) load(b + kLpWarps, ahead);
             m = LpVec<float>::max_nan(Vec::top(v[0]), Vec::top(v[1]));
+            lane_top = fmaxf(lane_top, m);   // a NaN loses
             asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
             const float y = m * scale;
             if (!(y <= ref + 8.f)) {
@@ -328,6 +367,21 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         }
     }
     count.settle();
+    const int busy = min(kLpWarps, block1 - block0);   // warps with blocks
+    if (p.top_k) {
+        // the lanes' maxima of the warp in descending order: its ceil(top_k / busy)-th.  No smaller one of all warps is needed.
+        uint32_t key = lp_key(lane_top);
+#pragma unroll
+        for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+            for (int d = size >> 1; d; d >>= 1) {   // bitonic
+                const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
+                const bool keep_large = ((lane & size) == 0) == ((lane & d) == 0);
+                key = keep_large ? max(key, o) : min(key, o);
+            }
+        key = __shfl_sync(0xffffffffu, key, busy ? (p.top_k + busy - 1) / busy - 1 : 0);
+        if (lane == 0) sh.bounds[warp] = lp_unkey(key);
+    }
     {
         LpSum mine;
         float a, b, c, d;
@@ -343,64 +397,76 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         mine.above = __reduce_add_sync(0xffffffffu, count.n);
         if (lane == 0) sh.sums[warp] = mine;
     }
+    if (threadIdx.x == 0) sh.found = 0;
     __syncthreads();
 
-    // ---- alternatives of the part: a list per warp, merged
+    // ---- alternatives of the part
     if (p.top_k) {
-        // the top_k-th largest of the lanes' maxima over all blocks: at least top_k values are as large
-        float bound = -INFINITY;
-        for (int i = lane; i < entries * kLpWarps; i += 32) bound = fmaxf(bound, sh.maxima[i]);   // a NaN loses
-        uint32_t key = lp_key(bound);
+        float bound = sh.bounds[0];
+        for (int w = 1; w < busy; ++w) bound = fminf(bound, sh.bounds[w]);
+        // what reaches the bound, in any order
+        const auto every_block = [&](auto&& take) {
+            for (int e = 0; e < entries; ++e) {
+                if (sh.maxima[e * kLpWarps + warp] < bound) continue;   // not for NaN
+                for (int i = e * shared_by; i < min(rounds, (e + 1) * shared_by); ++i) {
+                    const int b = block0 + i * kLpWarps + warp;
+                    if (b >= block1) break;
+                    load(b, v);
 #pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-            for (int d = size >> 1; d; d >>= 1) {   // bitonic, descending
-                const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
-                const bool keep_large = ((lane & size) == 0) == ((lane & d) == 0);
-                key = keep_large ? max(key, o) : min(key, o);
-            }
-        bound = lp_unkey(__shfl_sync(0xffffffffu, key, p.top_k - 1));
-        unsigned long long list = 0, least = 0;   // the lane's entry; the top_k-th
-        for (int e = 0; e < entries; ++e) {
-            const float m = sh.maxima[e * kLpWarps + warp];
-            if (m < bound) continue;   // not for NaN
-            for (int i = e * shared_by; i < min(rounds, (e + 1) * shared_by); ++i) {
-                const int b = block0 + i * kLpWarps + warp;
-                if (b >= block1) break;
-                load(b, v);
-#pragma unroll
-                for (int k = 0; k < kLpVecs; ++k) {
-                    if (!__any_sync(0xffffffffu, !(Vec::top(v[k]) < bound))) continue;
-                    float x[Vec::n];
-                    Vec::values(v[k], x);
-#pragma unroll 1
-                    for (int n = 0; n < Vec::n; ++n) {
-                        float mine = x[0];
-#pragma unroll
-                        for (int t = 1; t < Vec::n; ++t) mine = n == t ? x[t] : mine;
-                        const long long at = (long long)b * kBlock - skip + (k * 32 + lane) * Vec::n + n;
-                        const unsigned long long c = mine >= bound && at >= 0 && at < p.vocab ? ((unsigned long long)lp_key(mine) << 32) | (0xffffffffu - uint32_t(at)) : 0;
-                        for (uint32_t todo = __ballot_sync(0xffffffffu, c > least); todo; todo &= todo - 1) {
-                            const unsigned long long in = __shfl_sync(0xffffffffu, c, __ffs(todo) - 1);
-                            if (in <= least) continue;
-                            const int place = __popc(__ballot_sync(0xffffffffu, list > in));
-                            const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
-                            list = lane < place ? list : lane == place ? in : before;
-                            least = __shfl_sync(0xffffffffu, list, p.top_k - 1);
-                        }
-                    }
+                    for (int k = 0; k < kLpVecs; ++k) take(v[k], (long long)b * kBlock - skip + (k * 32 + lane) * Vec::n);
                 }
             }
-        }
-        sh.lists[warp][lane] = list;
-        if (warp == 0) sh.part.top[lane] = 0;
+        };
+        every_block([&](const uint4& vec, long long at) {
+            float x[Vec::n];
+            Vec::values(vec, x);
+            uint32_t hits = 0;
+#pragma unroll
+            for (int n = 0; n < Vec::n; ++n) hits |= x[n] >= bound ? 1u << n : 0u;
+            for (; hits; hits &= hits - 1) {   // seldom more than one lane's
+                const long long i = at + __ffs(hits) - 1;
+                if (i < 0 || i >= p.vocab) continue;
+                const int to = atomicAdd(&sh.found, 1);
+                if (to < kLpCandidates) sh.keys[to] = lp_entry(lp_value(row, i), i);
+            }
+        });
         __syncthreads();
-        lp_merge([&](int l) { return sh.lists[l]; }, kLpWarps, p.top_k, sh.part.top);
+        const int found = sh.found;
+        if (found > kLpCandidates) {
+            // many equal values: every warp keeps a sorted list of 32 across its lanes instead
+            __syncthreads();
+            unsigned long long list = 0, least = 0;   // the lane's entry; the top_k-th
+            every_block([&](const uint4& vec, long long at) {
+                if (!__any_sync(0xffffffffu, !(Vec::top(vec) < bound))) return;
+                float x[Vec::n];
+                Vec::values(vec, x);
+#pragma unroll 1
+                for (int n = 0; n < Vec::n; ++n) {
+                    float mine = x[0];
+#pragma unroll
+                    for (int t = 1; t < Vec::n; ++t) mine = n == t ? x[t] : mine;
+                    const unsigned long long key = mine >= bound && at + n >= 0 && at + n < p.vocab ? lp_entry(mine, at + n) : 0;
+                    for (uint32_t todo = __ballot_sync(0xffffffffu, key > least); todo; todo &= todo - 1) {
+                        const unsigned long long in = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
+                        if (in <= least) continue;
+                        const int place = __popc(__ballot_sync(0xffffffffu, list > in));
+                        const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
+                        list = lane < place ? list : lane == place ? in : before;
+                        least = __shfl_sync(0xffffffffu, list, p.top_k - 1);
+                    }
+                }
+            });
+            sh.keys[threadIdx.x] = list;
+            if (threadIdx.x < kLpMaxTop) sh.part.top[threadIdx.x] = 0;
+            __syncthreads();
+            lp_merge(sh.keys, kLpWarps, p.top_k, sh.part.top);
+        } else {
+            lp_rank(sh.keys, found, p.top_k, sh.part.top);
+        }
     }
-    if (threadIdx.x == 0) {
-        LpSum all = sh.sums[0];
-        for (int w = 1; w < kLpWarps; ++w) all = lp_join(all, sh.sums[w]);
-        sh.part.sum = all;
+    if (warp == kLpWarps - 1) {
+        const LpSum all = lp_join_lanes(sh.sums[lane & 7]);
+        if (lane == 0) sh.part.sum = all;
     }
 
     // ---- the parts of the row
@@ -408,8 +474,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
     if (p.parts > 1) cluster.sync();
     else __syncthreads();
     const auto part_of = [&](int c) -> const LpPart& { return p.parts > 1 ? *cluster.map_shared_rank(&sh.part, c) : sh.part; };
-    LpSum all = part_of(0).sum;
-    for (int c = 1; c < p.parts; ++c) all = lp_join(all, part_of(c).sum);
+    const auto all_parts = [&] {   // a lane asks for each part's sum; lanes without a part have a sum of nothing
+        LpSum v{-kLpHuge, 0.f, 0.f, -INFINITY, 0, 0};
+        if ((lane & 7) < p.parts) v = part_of(lane & 7).sum;
+        return p.parts > 1 ? lp_join_lanes(v) : sh.part.sum;
+    };
+    LpSum all = all_parts();
     const bool empty = all.top == -INFINITY && !all.nan;   // a row of -inf
     const bool huge = !all.nan && !empty && !(fabsf(all.top) <= kLpHuge && fabsf(all.top) * scale <= kLpFar);
     if (huge) {
@@ -432,12 +502,12 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         __syncthreads();
         if (threadIdx.x == 0) {
             for (int k = 1; k < kLpWarps; ++k) s += sh.sums[k].s, w += sh.sums[k].w;
-            sh.part.sum.s = s, sh.part.sum.w = w;
+            sh.part.sum.s = s, sh.part.sum.w = w, sh.part.sum.ref = 0.f;   // all against the same maximum
         }
         if (p.parts > 1) cluster.sync();
         else __syncthreads();
-        all.s = part_of(0).sum.s, all.w = part_of(0).sum.w;
-        for (int c = 1; c < p.parts; ++c) all.s += part_of(c).sum.s, all.w += part_of(c).sum.w;
+        const LpSum again = all_parts();
+        all.s = again.s, all.w = again.w;
     }
     if (part == 0) {
         const float log2_s = log2f(all.s);
@@ -457,14 +527,15 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
             if (p.entropy) p.entropy[r] = all.nan || isnan(all.s) ? NAN : empty ? 0.f : fmaxf(0.f, (log2_s - all.w / all.s) * kLn2);
         }
         if (p.top_k) {
-            // sh.lists is free: every warp of this CTA has come through the barrier above
             const unsigned long long* result = sh.part.top;
             if (p.parts > 1) {
-                if (threadIdx.x < kLpMaxTop) sh.lists[0][threadIdx.x] = 0;
+                // the candidates' place is free: every warp of this CTA has come through the barrier above
+                if (warp == 0) sh.out[lane] = 0;
+                if (warp < p.parts) sh.keys[threadIdx.x] = lane < p.top_k ? part_of(warp).top[lane] : 0;
                 __syncthreads();
-                lp_merge([&](int l) { return part_of(l).top; }, p.parts, p.top_k, sh.lists[0]);
+                lp_merge(sh.keys, p.parts, p.top_k, sh.out);
                 __syncthreads();
-                result = sh.lists[0];
+                result = sh.out;
             }
             if (int(threadIdx.x) < p.top_k) {
                 const unsigned long long key = result[threadIdx.x];

@@ -99,31 +99,33 @@ class ChunkAttention:
         need = ctypes.c_size_t(0)
         check(lib().garnet_b200_attention_chunk_workspace(ctypes.byref(self.opt), max_tokens, ctypes.byref(need)))
         self.ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
+        # what every call needs, at hand: the host side of a small call takes longer than its kernels
+        self._call, self._opt, self._ws, self._ws_bytes = lib().garnet_b200_attention_chunk, ctypes.byref(self.opt), self.ws.data_ptr(), need.value
+        self._dims = (cfg.qkv_width, (cfg.head_dim,), cfg.head_dim // 2, rope_positions, (cfg.page_size, cfg.kv_heads, cfg.head_dim),
+                      max_logical_pages, cfg.q_heads * cfg.head_dim)
 
     def run(self, qkv, q_norm_w, k_norm_w, cos, sin, key_pages, value_pages, page_tables, positions, row_starts, out, pdl: bool = False):
-        o, bf, i32 = self.opt, torch.bfloat16, torch.int32
-        on_device(qkv, "qkv", bf, (None, (o.q_heads + 2 * o.kv_heads) * o.head_dim))
-        batch, rows = positions.numel(), qkv.shape[0]
-        for w, name in ((q_norm_w, "q_norm_w"), (k_norm_w, "k_norm_w")):
-            on_device(w, name, bf, (o.head_dim,))
+        bf, i32, d = torch.bfloat16, torch.int32, self._dims
+        rows, batch, pages = qkv.shape[0], positions.numel(), key_pages.shape[0]
+        on_device(qkv, "qkv", bf, (rows, d[0]))
+        on_device(q_norm_w, "q_norm_w", bf, d[1])
+        on_device(k_norm_w, "k_norm_w", bf, d[1])
         for t, name in ((cos, "cos"), (sin, "sin")):
-            on_device(t, name, torch.float32, (None, o.head_dim // 2))
-            if t.shape[0] < o.rope_positions:
-                raise ValueError(f"{name} has fewer than {o.rope_positions} rows")
-        on_device(key_pages, "key_pages", bf, (None, o.page_size, o.kv_heads, o.head_dim))
-        on_device(value_pages, "value_pages", bf, tuple(key_pages.shape))
-        on_device(page_tables, "page_tables", i32, (batch, o.max_logical_pages))
+            on_device(t, name, torch.float32, (t.shape[0], d[2]))
+            if t.shape[0] < d[3]:
+                raise ValueError(f"{name} has fewer than {d[3]} rows")
+        on_device(key_pages, "key_pages", bf, (pages, *d[4]))
+        on_device(value_pages, "value_pages", bf, (pages, *d[4]))
+        on_device(page_tables, "page_tables", i32, (batch, d[5]))
         on_device(positions, "positions", i32, (batch,))
         on_device(row_starts, "row_starts", i32, (batch + 1,))
-        on_device(out, "out", bf, (rows, o.q_heads * o.head_dim))
-        if self.ws.device != qkv.device:
+        on_device(out, "out", bf, (rows, d[6]))
+        if self.ws.get_device() != qkv.get_device():
             raise ValueError("the workspace is on another device than the rows")
         if batch and rows:
-            check(lib().garnet_b200_attention_chunk(ctypes.byref(o), qkv.data_ptr(), q_norm_w.data_ptr(), k_norm_w.data_ptr(),
-                                                    cos.data_ptr(), sin.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
-                                                    page_tables.data_ptr(), positions.data_ptr(), row_starts.data_ptr(), out.data_ptr(),
-                                                    self.ws.data_ptr(), self.ws.numel(), batch, rows, key_pages.shape[0],
-                                                    1 if pdl else 0, stream_ptr()))
+            check(self._call(self._opt, qkv.data_ptr(), q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                             key_pages.data_ptr(), value_pages.data_ptr(), page_tables.data_ptr(), positions.data_ptr(),
+                             row_starts.data_ptr(), out.data_ptr(), self._ws, self._ws_bytes, batch, rows, pages, 1 if pdl else 0, stream_ptr()))
         return out
 
 
@@ -153,22 +155,29 @@ _LOGIT_KIND = {torch.float16: FP16, torch.bfloat16: BF16, torch.float32: FP32}
 def log_probs(logits, targets=None, top_k: int = 0, temperature: float = 1.0, pdl: bool = False) -> LogProbs:
     """Log probability and rank of the token targets[r] (int32) under softmax(logits[r] / temperature), the row's entropy and its top_k
     tokens, for logits [rows, vocab] of fp32, bf16 or fp16 (rows may lie further apart than vocab)."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _LOGIT_KIND:
+    kind = _LOGIT_KIND.get(logits.dtype) if isinstance(logits, torch.Tensor) and logits.dim() == 2 else None
+    if kind is None:
         raise ValueError("log_probs needs logits [rows, vocab] of fp32, bf16 or fp16")
     rows, vocab = logits.shape
-    stride = logits.stride(0) if rows > 1 else vocab
-    if not logits.is_cuda or logits.device.index != torch.cuda.current_device() or (vocab > 1 and logits.stride(1) != 1) or stride < vocab:
+    stride, step = logits.stride()
+    if rows <= 1:
+        stride = vocab
+    device = logits.device
+    if device.type != "cuda" or device.index != torch.cuda.current_device() or (vocab > 1 and step != 1) or stride < vocab:
         raise ValueError("log_probs needs rows of neighbouring values on the current CUDA device")
+    f32, i32, k = torch.float32, torch.int32, max(0, top_k)
+    log_prob = rank = None
     if targets is not None:
-        on_device(targets, "targets", torch.int32, (rows,))
-    f32, i32 = dict(dtype=torch.float32, device=logits.device), dict(dtype=torch.int32, device=logits.device)
-    r = LogProbs(None if targets is None else torch.empty(rows, **f32), None if targets is None else torch.empty(rows, **i32),
-                 torch.empty(rows, **f32), torch.empty(rows, max(0, top_k), **f32), torch.empty(rows, max(0, top_k), **i32))
+        on_device(targets, "targets", i32, (rows,))
+        log_prob, rank = torch.empty(rows, dtype=f32, device=device), torch.empty(rows, dtype=i32, device=device)
+    r = LogProbs(log_prob, rank, torch.empty(rows, dtype=f32, device=device), torch.empty(rows, k, dtype=f32, device=device),
+                 torch.empty(rows, k, dtype=i32, device=device))
     if rows:
-        ptr = lambda t: None if t is None or not t.numel() else t.data_ptr()   # noqa: E731
-        check(lib().garnet_b200_log_probs(logits.data_ptr(), _LOGIT_KIND[logits.dtype], stride, ptr(targets), rows, vocab, top_k, temperature,
-                                          ptr(r.log_probs), ptr(r.ranks), ptr(r.entropy), ptr(r.top_log_probs), ptr(r.top_ids),
-                                          1 if pdl else 0, stream_ptr()))
+        given = targets is not None
+        check(lib().garnet_b200_log_probs(logits.data_ptr(), kind, stride, targets.data_ptr() if given else None, rows, vocab, top_k, temperature,
+                                          log_prob.data_ptr() if given else None, rank.data_ptr() if given else None, r.entropy.data_ptr(),
+                                          r.top_log_probs.data_ptr() if k else None, r.top_ids.data_ptr() if k else None, 1 if pdl else 0,
+                                          stream_ptr()))
     return r
 
 
