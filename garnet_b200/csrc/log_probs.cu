@@ -3,12 +3,13 @@
 //   y = x log2(e) / T, a reference r near the row's maximum of y, S = sum 2^(y - r), W = sum 2^(y - r) (y - r):
 //   log p(t) = ln 2 ((y_t - r) - log2 S),  H = ln 2 (log2 S - W / S),  rank = 1 + #{x > x_t}.
 //
-// A row is cut into 1, 2, 4 or 8 parts, one CTA each, that meet through distributed shared memory.  The warps of a CTA take blocks of 1 KB in
-// turn: two 16-byte loads per lane, the block's maximum (NaN wins) by packed maxima and one warp reduction, which also says whether the
+// A row is cut into 1, 2, 4 or 8 parts, one CTA each, that meet through distributed shared memory.  The warps of a CTA take blocks of 2 KB in
+// turn: four 16-byte loads per lane, the block's maximum (NaN wins) by packed maxima and one warp reduction, which also says whether the
 // warp's reference has to grow (by more than 2^8, so that this is rare: S and W are rescaled then), then per value one conversion,
-// half of a packed multiply-add, one exponential and half of two packed additions; the rank is counted in packed 16-bit numbers.
-// The block maxima stay in shared memory.  With n warps the ceil(top_k / n)-th largest of a warp's 32 lane maxima, of all warps the least, is
-// no larger than the top_k-th largest logit, so that only blocks that reach it are read a second time (from L2) for the alternatives: every
+// half of a packed multiply-add, one exponential and half of two packed additions; the rank is counted in packed 16-bit numbers,
+// in blocks whose maximum is above the target's logit.
+// The block maxima stay in shared memory.  The top_k-th largest of the threads' own maxima is no larger than the top_k-th
+// largest logit, so that only blocks that reach it - few more than top_k - are read a second time (from L2) for the alternatives: every
 // value that reaches it becomes a candidate, (value, lowest index) as one 64-bit number, and the candidates larger than it say its place.
 // Where too many are equal for that, every warp keeps a sorted list across its lanes.
 // Everything is added in an order that depends on sizes only.  A row whose maximum lies beyond +-2^100 (a mask of the type's lowest
@@ -28,10 +29,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32, kLpMaxParts = 8;
-constexpr int kLpCandidates = 256;
-constexpr int kLpVecs = 2, kLpBlockBytes = kLpVecs * 32 * 16;
+constexpr int kLpVecs = 4, kLpBlockBytes = kLpVecs * 32 * 16;
 constexpr int kLpEntries = 128;   // block maxima that a warp keeps; more blocks share them
 constexpr float kLpHuge = 1.2676506002282294e30f;   // 2^100
 constexpr float kLpFar = 1048576.f;                 // 2^20: the reference, an fp32 number, is then within 2^-4 of the y that it stands for
@@ -106,7 +105,7 @@ struct LpPairs {
     }
     // values with -inf and what lies below -2^100 as -2^100
     __device__ static void finite(const uint4& v, float (&x)[8]);
-    // counted as 16-bit floating-point numbers: exact up to 256, and a block adds at most 8 to either half
+    // counted as 16-bit floating-point numbers: exact up to 256, and a vector adds at most 4 to either half
     struct Count {
         int n = 0;
         T2 than, halves;
@@ -149,14 +148,6 @@ struct LpVec<__half> : LpPairs<__half2> {};
 __device__ __forceinline__ float lp_value(const float* x, long long i) { return x[i]; }
 __device__ __forceinline__ float lp_value(const __nv_bfloat16* x, long long i) { return __bfloat162float(x[i]); }
 __device__ __forceinline__ float lp_value(const __half* x, long long i) { return __half2float(x[i]); }
-__device__ __forceinline__ uint32_t lp_bits(const float* x, long long i) { return __float_as_uint(x[i]); }
-__device__ __forceinline__ uint32_t lp_bits(const __nv_bfloat16* x, long long i) { return reinterpret_cast<const uint16_t*>(x)[i]; }
-__device__ __forceinline__ uint32_t lp_bits(const __half* x, long long i) { return reinterpret_cast<const uint16_t*>(x)[i]; }
-
-// -inf
-__device__ __forceinline__ uint32_t lp_none(const float*) { return 0xff800000u; }
-__device__ __forceinline__ uint32_t lp_none(const __nv_bfloat16*) { return 0xff80u; }
-__device__ __forceinline__ uint32_t lp_none(const __half*) { return 0xfc00u; }
 
 // Larger for larger values, the same for +0 and -0; 0 for NaN.
 __device__ __forceinline__ uint32_t lp_key(float x)
@@ -205,14 +196,18 @@ struct LpPart {
     LpSum sum;
     unsigned long long top[kLpMaxTop];
 };
+template <int kThreads>
 struct LpShared {
+    static constexpr int warps = kThreads / 32, candidates = kThreads;
     LpPart part;
-    LpSum sums[kLpWarps];
-    int found;                                        // candidates in `keys`, or more than there is room for
-    unsigned long long keys[kLpCandidates];           // candidates in no order; or lists of 32, one per warp; or the parts' lists
+    LpSum sums[8];
+    int found;                                               // candidates in `keys`, or more than there is room for
+    unsigned long long keys[kLpMaxParts * kLpMaxTop];        // candidates in no order; or lists of 32, one per warp; or the parts' lists
     unsigned long long out[kLpMaxTop];
-    float bounds[kLpWarps];
-    float maxima[kLpEntries * kLpWarps];              // [entry][warp]
+    alignas(16) uint32_t lane_tops[kThreads];                // as keys
+    uint32_t bound;
+    float maxima[kLpEntries * warps];                        // [entry][warp]
+    static_assert(warps <= 8 && candidates <= kLpMaxParts * kLpMaxTop, "room for sums and keys");
 };
 
 // The largest `most` of `count` different keys, up to one per thread, to out[0 ..] in descending order; 0 where there are fewer.
@@ -229,159 +224,144 @@ __device__ __forceinline__ void lp_rank(const unsigned long long* keys, int coun
 
 // The same of `lists` descending lists of 32, which 0 may follow: a key's place is its place in its list and the numbers of larger keys in
 // the others.  Out's 32 entries are 0 before.
+template <int kThreads>
 __device__ __forceinline__ void lp_merge(const unsigned long long* keys, int lists, int most, unsigned long long* out)
 {
-    const int mine = threadIdx.x >> 5;
-    if (mine >= lists) return;
-    const unsigned long long key = keys[threadIdx.x];
-    int larger[kLpWarps] = {};
+    for (int i = threadIdx.x; i < lists * 32; i += kThreads) {
+        const unsigned long long key = keys[i];
+        int larger[kLpMaxParts] = {};
 #pragma unroll
-    for (int step = 16; step; step >>= 1)
+        for (int step = 16; step; step >>= 1)
 #pragma unroll
-        for (int l = 0; l < kLpWarps; ++l)
-            if (l < lists && keys[l * 32 + larger[l] + step - 1] > key) larger[l] += step;
-    int place = 0;
+            for (int l = 0; l < kLpMaxParts; ++l)
+                if (l < lists && keys[l * 32 + larger[l] + step - 1] > key) larger[l] += step;
+        int place = 0;
 #pragma unroll
-    for (int l = 0; l < kLpWarps; ++l) place += l < lists ? larger[l] + (larger[l] == 31 && keys[l * 32 + 31] > key) : 0;
-    if (key && place < most) out[place] = key;
+        for (int l = 0; l < kLpMaxParts; ++l) place += l < lists ? larger[l] + (larger[l] == 31 && keys[l * 32 + 31] > key) : 0;
+        if (key && place < most) out[place] = key;
+    }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs p)
+template <typename T, int kLpThreads>
+__global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kernel(const LogProbs p)
 {
     using Vec = LpVec<T>;
-    constexpr int kBlock = kLpBlockBytes / int(sizeof(T));
-    __shared__ LpShared sh;
+    constexpr int kBlock = kLpBlockBytes / int(sizeof(T)), kLpWarps = kLpThreads / 32, kLpCandidates = LpShared<kLpThreads>::candidates;
+    __shared__ LpShared<kLpThreads> sh;
     pdl_launch_dependents();
     pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int part = int(blockIdx.x) % p.parts;
     const size_t r = blockIdx.x / unsigned(p.parts);
     const T* row = static_cast<const T*>(p.logits) + r * p.stride;
-    // blocks start on 16-byte boundaries: value i of the row is value i + skip of its blocks
-    const int skip = int((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
-    const T* base = row - skip;
-    const int blocks = int(((long long)p.vocab + skip + kBlock - 1) / kBlock);
+    // whole blocks from the row's first 16-byte boundary on; the first part has the values before them, the last part those behind
+    const int head = min(p.vocab, int((16 - (reinterpret_cast<uintptr_t>(row) & 15)) % 16 / sizeof(T)));
+    const int blocks = (p.vocab - head) / kBlock, tail = head + blocks * kBlock;
     const int block0 = int((long long)part * blocks / p.parts), block1 = int((long long)(part + 1) * blocks / p.parts);
+    const int loose0 = part == 0 ? head : 0, loose = loose0 + (part + 1 == p.parts ? p.vocab - tail : 0);   // single values of this part
+    const auto loose_at = [&](int i) { return i < loose0 ? i : tail + i - loose0; };
+    const uint4* row_blocks = reinterpret_cast<const uint4*>(row + head) + lane;
+    const auto block_at = [&](int b) { return row_blocks + (long long)b * (kLpBlockBytes / 16); };
     const float scale = p.scale * 1.4426950408889634f;
 
-    // a lane's vectors of a block; what lies outside the row is -inf
-    const auto load = [&](int b, uint4 (&v)[kLpVecs]) {
-        const long long first = (long long)b * kBlock - skip;
-        const uint4* from = reinterpret_cast<const uint4*>(base + (long long)b * kBlock) + lane;
-        if (first >= 0 && first + kBlock <= p.vocab) {
-#pragma unroll
-            for (int k = 0; k < kLpVecs; ++k) v[k] = __ldg(from + 32 * k);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kLpVecs; ++k) {
-                const long long at = first + (k * 32 + lane) * Vec::n;
-                uint32_t w[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    constexpr int per = Vec::n / 4;
-                    const uint32_t none = lp_none(row);
-                    uint32_t bits = 0;
-#pragma unroll
-                    for (int h = 0; h < per; ++h) {
-                        const long long e = at + i * per + h;
-                        bits |= (e >= 0 && e < p.vocab ? lp_bits(row, e) : none) << (16 * h);
-                    }
-                    w[i] = bits;
-                }
-                v[k] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-        }
-    };
-
     const int rounds = (block1 - block0 + kLpWarps - 1) / kLpWarps;          // blocks of a warp
-    if (rounds > 1 && rounds <= 16) {
-        // a short part: all of it is asked for at once, eight lanes per block of 1 KB
-        for (int i = lane >> 3; i < rounds; i += 4) {
-            const long long at = (long long)(block0 + i * kLpWarps + warp) * kLpBlockBytes + (lane & 7) * 128;
-            if (block0 + i * kLpWarps + warp < block1 && at >= 0 && at < ((long long)p.vocab + skip) * int(sizeof(T)))
-                asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(base) + at));
-        }
+    if (rounds > 1 && rounds <= 8) {
+        // a short part: all of it is asked for at once, sixteen lanes per block of 2 KB
+        for (int i = lane >> 4; i < rounds; i += 2)
+            if (block0 + i * kLpWarps + warp < block1)
+                asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const char*>(row + head) + (long long)(block0 + i * kLpWarps + warp) * kLpBlockBytes + (lane & 15) * 128));
     }
-    const int shared_by = (rounds + kLpEntries - 1) / kLpEntries, entries = (rounds + shared_by - 1) / shared_by;
+    const int shared_by = max(1, (rounds + kLpEntries - 1) / kLpEntries), entries = (rounds + shared_by - 1) / shared_by;
     float ref = -kLpHuge * scale, entry = -INFINITY, top = -INFINITY, lane_top = -INFINITY;   // ref: in powers of two
     int nan = 0;
     uint64_t s2[2] = {0, 0}, w2[2] = {0, 0};
     const uint64_t scale2 = f32x2(scale, scale);
-    uint4 v[kLpVecs], ahead[kLpVecs];
-    if (block0 + warp < block1) load(block0 + warp, ahead);   // asked for before the two dependent loads of the target's logit
+    uint4 v[kLpVecs];
+    int b = block0 + warp;
+    const uint4* from = block_at(b);
+    if (b < block1) {   // asked for before the two dependent loads of the target's logit
+#pragma unroll
+        for (int k = 0; k < kLpVecs; ++k) v[k] = __ldg(from + 32 * k);
+    }
     const int target = p.targets ? p.targets[r] : -1;
     const bool given = target >= 0 && target < p.vocab;
     const float x_t = given ? lp_value(row, target) : INFINITY;
     typename Vec::Count count(x_t);
-    for (int i = 0; i < rounds; ++i) {
-        const int b = block0 + i * kLpWarps + warp;
-        float m = -INFINITY;
-        if (b < block1) {
+    // the warp's reference grows to its new maximum m (a NaN is noted)
+    const auto grow = [&](float m) {
+        const float y = m * scale;
+        if (y <= ref + 8.f) return;
+        if (isnan(m)) {
+            nan = 1;
+        } else if (m <= kLpHuge) {   // beyond that the row is summed again
+            const float d = ref - y, f = ex2(d);
+            const uint64_t f2 = f32x2(f, f), d2 = f32x2(fmaxf(d, -1e30f), fmaxf(d, -1e30f));
 #pragma unroll
-            for (int k = 0; k < kLpVecs; ++k) v[k] = ahead[k];
-            if (b + kLpWarps < block1) load(b + kLpWarps, ahead);
-            m = LpVec<float>::max_nan(Vec::top(v[0]), Vec::top(v[1]));
-            lane_top = fmaxf(lane_top, m);   // a NaN loses
-            asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
-            const float y = m * scale;
-            if (!(y <= ref + 8.f)) {
-                if (isnan(m)) {
-                    nan = 1;
-                } else if (m <= kLpHuge) {   // beyond that the row is summed again
-                    const float d = ref - y, f = ex2(d);
-                    const uint64_t f2 = f32x2(f, f), d2 = f32x2(fmaxf(d, -1e30f), fmaxf(d, -1e30f));
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        w2[k] = mul2(f2, fma2(d2, s2[k], w2[k]));
-                        s2[k] = mul2(f2, s2[k]);
-                    }
-                    ref = y;
-                }
+            for (int k = 0; k < 2; ++k) {
+                w2[k] = mul2(f2, fma2(d2, s2[k], w2[k]));
+                s2[k] = mul2(f2, s2[k]);
             }
-            const uint64_t minus2 = f32x2(-ref, -ref);
-#pragma unroll
-            for (int k = 0; k < kLpVecs; ++k) {
-                float x[Vec::n];
-                Vec::finite(v[k], x);
-                count.add(v[k]);
-#pragma unroll
-                for (int e = 0; e < Vec::n; e += 2) {
-                    const uint64_t d = fma2(f32x2(x[e], x[e + 1]), scale2, minus2);
-                    float a, c;
-                    f32x2_split(d, a, c);
-                    const uint64_t p2 = f32x2(ex2(a), ex2(c));
-                    s2[(e >> 1) & 1] = add2(s2[(e >> 1) & 1], p2);
-                    w2[(e >> 1) & 1] = fma2(p2, d, w2[(e >> 1) & 1]);
-                }
-            }
-            if ((i & 31) == 31) count.settle();
+            ref = y;
         }
-        // a block with a NaN counts as one that may hold alternatives, and not for the bound on them
-        if (isnan(m)) entry = m;
-        else if (!isnan(entry)) entry = fmaxf(entry, m);
+    };
+    float* to = sh.maxima + warp;
+    int left = shared_by, unsettled = 256 / (2 * Vec::n * kLpVecs / 4);
+#pragma unroll 1
+    for (; b < block1; b += kLpWarps) {
+        float m = Vec::top(v[0]);
+#pragma unroll
+        for (int k = 1; k < kLpVecs; ++k) m = LpVec<float>::max_nan(m, Vec::top(v[k]));
+        lane_top = fmaxf(lane_top, m);   // a NaN loses
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+        grow(m);
+        if (m > x_t) {   // else none of the block is larger than the target's; a row with a NaN needs no rank
+#pragma unroll
+            for (int k = 0; k < kLpVecs; ++k) count.add(v[k]);
+        }
+        const uint64_t minus2 = f32x2(-ref, -ref);
+        if (b + kLpWarps < block1) from += kLpWarps * (kLpBlockBytes / 16);   // the last block is asked for twice
+#pragma unroll
+        for (int k = 0; k < kLpVecs; ++k) {
+            float x[Vec::n];
+            Vec::finite(v[k], x);
+            v[k] = __ldg(from + 32 * k);
+#pragma unroll
+            for (int e = 0; e < Vec::n; e += 2) {
+                const uint64_t d = fma2(f32x2(x[e], x[e + 1]), scale2, minus2);
+                float a, c;
+                f32x2_split(d, a, c);
+                const uint64_t p2 = f32x2(ex2(a), ex2(c));
+                s2[(e >> 1) & 1] = add2(s2[(e >> 1) & 1], p2);
+                w2[(e >> 1) & 1] = fma2(p2, d, w2[(e >> 1) & 1]);
+            }
+        }
+        if (--unsettled == 0) {
+            count.settle();
+            unsettled = 256 / (2 * Vec::n * kLpVecs / 4);
+        }
+        entry = LpVec<float>::max_nan(entry, m);   // a block with a NaN counts as one that may hold alternatives
         top = fmaxf(top, m);
-        if ((i + 1) % shared_by == 0 || i + 1 == rounds) {
-            if (lane == 0) sh.maxima[i / shared_by * kLpWarps + warp] = entry;
-            entry = -INFINITY;
+        if (--left == 0) {
+            if (lane == 0) *to = entry;
+            to += kLpWarps;
+            left = shared_by, entry = -INFINITY;
         }
+    }
+    if (lane == 0 && to < sh.maxima + entries * kLpWarps) *to = entry;
+    for (int i0 = warp * 32; i0 < loose; i0 += kLpThreads) {
+        const float x = i0 + lane < loose ? lp_value(row, loose_at(i0 + lane)) : -INFINITY;
+        float m = x;
+        lane_top = fmaxf(lane_top, x);
+        asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
+        grow(m);
+        top = fmaxf(top, m);
+        count.n += x > x_t;
+        const float d = fmaf(fmaxf(x, -kLpHuge), scale, -ref), e = i0 + lane < loose ? ex2(d) : 0.f;
+        s2[0] = add2(s2[0], f32x2(e, 0.f));
+        w2[0] = fma2(f32x2(e, 0.f), f32x2(d, 0.f), w2[0]);
     }
     count.settle();
-    const int busy = min(kLpWarps, block1 - block0);   // warps with blocks
-    if (p.top_k) {
-        // the lanes' maxima of the warp in descending order: its ceil(top_k / busy)-th.  No smaller one of all warps is needed.
-        uint32_t key = lp_key(lane_top);
-#pragma unroll
-        for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll
-            for (int d = size >> 1; d; d >>= 1) {   // bitonic
-                const uint32_t o = __shfl_xor_sync(0xffffffffu, key, d);
-                const bool keep_large = ((lane & size) == 0) == ((lane & d) == 0);
-                key = keep_large ? max(key, o) : min(key, o);
-            }
-        key = __shfl_sync(0xffffffffu, key, busy ? (p.top_k + busy - 1) / busy - 1 : 0);
-        if (lane == 0) sh.bounds[warp] = lp_unkey(key);
-    }
+    if (p.top_k) sh.lane_tops[threadIdx.x] = lp_key(lane_top);
     {
         LpSum mine;
         float a, b, c, d;
@@ -397,13 +377,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         mine.above = __reduce_add_sync(0xffffffffu, count.n);
         if (lane == 0) sh.sums[warp] = mine;
     }
-    if (threadIdx.x == 0) sh.found = 0;
+    if (threadIdx.x == 0) sh.found = 0, sh.bound = 0xffffffffu;
     __syncthreads();
 
     // ---- alternatives of the part
     if (p.top_k) {
-        float bound = sh.bounds[0];
-        for (int w = 1; w < busy; ++w) bound = fminf(bound, sh.bounds[w]);
+        // the top_k-th largest of the threads' maxima
+        const uint32_t mine = lp_key(lane_top);
+        int larger = 0;
+#pragma unroll 8
+        for (int i = 0; i < kLpThreads; i += 4) {
+            const uint4 o = *reinterpret_cast<const uint4*>(&sh.lane_tops[i]);
+            larger += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+        }
+        if (larger < p.top_k) atomicMin(&sh.bound, mine);
+        __syncthreads();
+        const float bound = sh.bound ? lp_unkey(sh.bound) : -INFINITY;
         // what reaches the bound, in any order
         const auto every_block = [&](auto&& take) {
             for (int e = 0; e < entries; ++e) {
@@ -411,32 +400,48 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
                 for (int i = e * shared_by; i < min(rounds, (e + 1) * shared_by); ++i) {
                     const int b = block0 + i * kLpWarps + warp;
                     if (b >= block1) break;
-                    load(b, v);
 #pragma unroll
-                    for (int k = 0; k < kLpVecs; ++k) take(v[k], (long long)b * kBlock - skip + (k * 32 + lane) * Vec::n);
+                    for (int k = 0; k < kLpVecs; ++k) v[k] = __ldg(block_at(b) + 32 * k);
+#pragma unroll
+                    for (int k = 0; k < kLpVecs; ++k) take(v[k], head + b * kBlock + (k * 32 + lane) * Vec::n);
                 }
             }
         };
-        every_block([&](const uint4& vec, long long at) {
+        const auto candidate = [&](float x, int i) {
+            const int to = atomicAdd(&sh.found, 1);
+            if (to < kLpCandidates) sh.keys[to] = lp_entry(x, i);
+        };
+        every_block([&](const uint4& vec, int at) {
             float x[Vec::n];
             Vec::values(vec, x);
             uint32_t hits = 0;
 #pragma unroll
             for (int n = 0; n < Vec::n; ++n) hits |= x[n] >= bound ? 1u << n : 0u;
             for (; hits; hits &= hits - 1) {   // seldom more than one lane's
-                const long long i = at + __ffs(hits) - 1;
-                if (i < 0 || i >= p.vocab) continue;
-                const int to = atomicAdd(&sh.found, 1);
-                if (to < kLpCandidates) sh.keys[to] = lp_entry(lp_value(row, i), i);
+                const int i = at + __ffs(hits) - 1;
+                candidate(lp_value(row, i), i);
             }
         });
+        for (int i = threadIdx.x; i < loose; i += kLpThreads)
+            if (lp_value(row, loose_at(i)) >= bound) candidate(lp_value(row, loose_at(i)), loose_at(i));
         __syncthreads();
         const int found = sh.found;
         if (found > kLpCandidates) {
             // many equal values: every warp keeps a sorted list of 32 across its lanes instead
             __syncthreads();
             unsigned long long list = 0, least = 0;   // the lane's entry; the top_k-th
-            every_block([&](const uint4& vec, long long at) {
+            const auto keep = [&](float x, int i) {
+                const unsigned long long key = x >= bound ? lp_entry(x, i) : 0;
+                for (uint32_t todo = __ballot_sync(0xffffffffu, key > least); todo; todo &= todo - 1) {
+                    const unsigned long long in = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
+                    if (in <= least) continue;
+                    const int place = __popc(__ballot_sync(0xffffffffu, list > in));
+                    const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
+                    list = lane < place ? list : lane == place ? in : before;
+                    least = __shfl_sync(0xffffffffu, list, p.top_k - 1);
+                }
+            };
+            every_block([&](const uint4& vec, int at) {
                 if (!__any_sync(0xffffffffu, !(Vec::top(vec) < bound))) return;
                 float x[Vec::n];
                 Vec::values(vec, x);
@@ -445,27 +450,24 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
                     float mine = x[0];
 #pragma unroll
                     for (int t = 1; t < Vec::n; ++t) mine = n == t ? x[t] : mine;
-                    const unsigned long long key = mine >= bound && at + n >= 0 && at + n < p.vocab ? lp_entry(mine, at + n) : 0;
-                    for (uint32_t todo = __ballot_sync(0xffffffffu, key > least); todo; todo &= todo - 1) {
-                        const unsigned long long in = __shfl_sync(0xffffffffu, key, __ffs(todo) - 1);
-                        if (in <= least) continue;
-                        const int place = __popc(__ballot_sync(0xffffffffu, list > in));
-                        const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
-                        list = lane < place ? list : lane == place ? in : before;
-                        least = __shfl_sync(0xffffffffu, list, p.top_k - 1);
-                    }
+                    keep(mine, at + n);
                 }
             });
+            for (int i0 = warp * 32; i0 < loose; i0 += kLpThreads) {
+                const bool there = i0 + lane < loose;
+                const int i = there ? loose_at(i0 + lane) : 0;
+                keep(there ? lp_value(row, i) : NAN, i);
+            }
             sh.keys[threadIdx.x] = list;
             if (threadIdx.x < kLpMaxTop) sh.part.top[threadIdx.x] = 0;
             __syncthreads();
-            lp_merge(sh.keys, kLpWarps, p.top_k, sh.part.top);
+            lp_merge<kLpThreads>(sh.keys, kLpWarps, p.top_k, sh.part.top);
         } else {
             lp_rank(sh.keys, found, p.top_k, sh.part.top);
         }
     }
     if (warp == kLpWarps - 1) {
-        const LpSum all = lp_join_lanes(sh.sums[lane & 7]);
+        const LpSum all = lp_join_lanes((lane & 7) < kLpWarps ? sh.sums[lane & 7] : LpSum{-kLpHuge, 0.f, 0.f, -INFINITY, 0, 0});
         if (lane == 0) sh.part.sum = all;
     }
 
@@ -487,12 +489,13 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         if (p.parts > 1) cluster.sync();   // the others have read this part's sums
         else __syncthreads();
         float s = 0.f, w = 0.f;
-        const long long from = max(0ll, (long long)block0 * kBlock - skip), to = min((long long)p.vocab, (long long)block1 * kBlock - skip);
-        for (long long i = from + threadIdx.x; i < to; i += kLpThreads) {
+        const auto add = [&](int i) {
             const float d = (lp_value(row, i) - all.top) * scale, e = ex2(d);
             s += e;
             w += e > 0.f ? e * d : 0.f;   // inf - inf is NaN, and s with it
-        }
+        };
+        for (int i = block0 * kBlock + int(threadIdx.x); i < block1 * kBlock; i += kLpThreads) add(head + i);
+        for (int i = threadIdx.x; i < loose; i += kLpThreads) add(loose_at(i));
 #pragma unroll
         for (int o = 16; o; o >>= 1) {
             s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -531,9 +534,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
             if (p.parts > 1) {
                 // the candidates' place is free: every warp of this CTA has come through the barrier above
                 if (warp == 0) sh.out[lane] = 0;
-                if (warp < p.parts) sh.keys[threadIdx.x] = lane < p.top_k ? part_of(warp).top[lane] : 0;
+                for (int c = warp; c < p.parts; c += kLpWarps) sh.keys[c * 32 + lane] = lane < p.top_k ? part_of(c).top[lane] : 0;
                 __syncthreads();
-                lp_merge(sh.keys, p.parts, p.top_k, sh.out);
+                lp_merge<kLpThreads>(sh.keys, p.parts, p.top_k, sh.out);
                 __syncthreads();
                 result = sh.out;
             }
@@ -545,6 +548,13 @@ __global__ void __launch_bounds__(kLpThreads, 4) log_probs_kernel(const LogProbs
         }
     }
     if (p.parts > 1) cluster.sync();   // the first part may still read this one
+}
+
+template <int kThreads>
+auto lp_kernel(int dtype)
+{
+    return dtype == GARNET_B200_BF16 ? log_probs_kernel<__nv_bfloat16, kThreads>
+           : dtype == GARNET_B200_FP16 ? log_probs_kernel<__half, kThreads> : log_probs_kernel<float, kThreads>;
 }
 
 }  // namespace
@@ -571,15 +581,16 @@ int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, c
     if (top_k < 0 || top_k > vocab || (top_k > 0 && (!d_top_log_probs || !d_top_ids)))
         return fail(GARNET_B200_INVALID_VALUE, "log_probs: bad top_k %d, or no arrays for it", top_k);
     if (top_k > kLpMaxTop) return fail(GARNET_B200_NOT_SUPPORTED, "log_probs: top_k above %d", kLpMaxTop);
-    // as many parts as run at once, four CTAs to an SM, each with a block for every warp
+    // few rows: as many parts as run at once, four CTAs of 256 threads to an SM, each with a block for every warp
     const long long blocks = (long long)vocab * (dtype == GARNET_B200_FP32 ? 4 : 2) / kLpBlockBytes;
     int parts = 1;
-    while (parts < kLpMaxParts && (long long)rows * parts * 2 <= 4 * kSmCount && blocks >= 2 * parts * kLpWarps) parts *= 2;
+    while (parts < kLpMaxParts && (long long)rows * parts * 2 <= 4 * kSmCount && blocks >= 2 * parts * 8) parts *= 2;
+    const int threads = rows > 4 * kSmCount ? 128 : 256;
     if ((long long)rows * parts > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "log_probs: too many rows");
     const LogProbs p{d_logits, row_stride, d_targets, d_log_probs, d_ranks, d_entropy, d_top_log_probs, d_top_ids, vocab, top_k, parts, 1.f / temperature};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(rows) * unsigned(parts));
-    cfg.blockDim = dim3(kLpThreads);
+    cfg.blockDim = dim3(unsigned(threads));
     cfg.stream = static_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -588,7 +599,7 @@ int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, c
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = (flags & 1u) ? 2 : 1;
-    GB_CUDA(cudaLaunchKernelEx(&cfg, dtype == GARNET_B200_BF16 ? log_probs_kernel<__nv_bfloat16> : dtype == GARNET_B200_FP16 ? log_probs_kernel<__half> : log_probs_kernel<float>, p));
+    GB_CUDA(cudaLaunchKernelEx(&cfg, threads == 128 ? lp_kernel<128>(dtype) : lp_kernel<256>(dtype), p));
     return GARNET_B200_OK;
 }
 
