@@ -2,12 +2,13 @@
 //
 // A CTA owns one kv head and one or two tiles of 128 query rows; a tile's rows are (token, q head of the group), so that the K and V
 // rows it stages serve all the q heads of the group.  Per step of 128 (or 64) keys:
-//   loader warp     looks up the pages of the step, one lane per box of rows that lie together in the cache, and copies K and V by TMA
-//                   into a ring of slots: two halves of 64 dims, 128-byte rows, swizzled - the K-major operand of Q K^T and the
-//                   MN-major operand of P V.  Rows that do not exist, and those behind the last key that a row of the CTA sees, come
-//                   from behind the end of the tensor, which reads as zeros (what the cache holds there could be NaN);
-//   MMA warp        one thread: P V of a step when its P is there, then Q K^T of the next step, tile by tile: the tensor pipe works on
-//                   one tile while the other tile's softmax runs;
+//   loader warps    look up the page of every key and copy its K and V rows by cp.async into a ring of slots: two halves of 64 dims,
+//                   128-byte rows, swizzled - the K-major operand of Q K^T and the MN-major operand of P V.  Rows that do not exist,
+//                   and those behind the last key that a row of the CTA sees, are filled with zeros (what the cache holds there
+//                   could be NaN).  TMA boxes of a page took the loader 120 clocks each to ask for (16 rows x 128 bytes; 4000 clocks
+//                   per step of 128 keys, more than all the rest);
+//   MMA warps       one thread per tile: P V of 32 keys when their P is there, after the last ones Q K^T of the next step: the tensor
+//                   pipe works on one tile while the other tile's softmax runs;
 //   softmax warps   one thread per query row: scores into registers, running maximum, p = 2^(s c - m c), the row's sum in fp32, P as
 //                   bf16 over the scores in tensor memory; O stays in tensor memory and is rescaled only when a row's maximum has
 //                   grown by more than 2^8 since the last time (the final division makes that exact; the conditional rescaling of
@@ -35,11 +36,14 @@ constexpr int kChMaxSplits = 8;
 
 template <int kTiles, int kKeys, int kSlots>
 struct ChShape {
-    static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, load_warp = mma_warp + 1, threads = (load_warp + 1) * 32;
+    // warps are allocated four at a time: 12 leave a thread 168 registers, twice 8 leave it 128
+    static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, load_warp = mma_warp + kTiles, loaders = 4 - kTiles;
+    static constexpr int threads = (load_warp + loaders) * 32;
+    static constexpr int chunks = kKeys / 32;   // P is handed over 32 keys at a time
     static constexpr int q_half = kChRows * 128, q_tile = 2 * q_half;    // 64 dims of a tile of queries; all of them
     static constexpr int half = kKeys * 128, slot = 2 * half;            // the same of a step's keys (or values)
     static constexpr int q = 0, ring = kTiles * q_tile, exists = ring + kSlots * slot, bars = exists + 4 * (kKeys / 32) * 4;
-    static constexpr int total = bars + 192 + 1024;                      // barriers, and slack for 1024-byte alignment
+    static constexpr int total = bars + 256 + 1024;                      // barriers, and slack for 1024-byte alignment
     // partial results of a split call, over the queries and the ring: rows of 128 floats, 16 bytes apart in the banks; maxima, sums
     static constexpr int part_row = (kChDim + 4) * 4, stats = kTiles * kChRows * part_row;
     static_assert(stats + kTiles * kChRows * 8 <= exists, "the partial results fit where the queries and the ring were");
@@ -47,12 +51,6 @@ struct ChShape {
     // tensor memory of a tile: the scores (P replaces them), O
     static constexpr uint32_t col_o = kKeys, tile_cols = kKeys + kChDim, cols = kTiles * tile_cols <= 256 ? 256 : 512;
     static_assert(kTiles * tile_cols <= 512, "tensor memory");
-};
-
-struct ChMaps {
-    CUtensorMap q;                // [kv head][token][q head of the group] rows of 128
-    CUtensorMap k, v;             // boxes of `box` cache rows of a kv head
-    CUtensorMap k_row, v_row;     // boxes of one row
 };
 
 // The query rows of a CTA: up to `rows` tokens of sequence b from its token `first` on.
@@ -97,7 +95,7 @@ __device__ __forceinline__ ChBlock chunk_block(const Chunk& p, int y, int rows, 
 
 template <int kTiles, int kKeys, int kSlots>
 __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTiles == 1 ? 2 : 1)
-    attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ ChMaps maps, const int box, const int splits)
+    attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
 {
     using S = ChShape<kTiles, kKeys, kSlots>;
     extern __shared__ uint8_t smem_raw[];
@@ -107,10 +105,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     uint64_t* empty = full + kSlots;                                        // [slots]
     uint64_t* q_full = empty + kSlots;
     uint64_t* s_full = q_full + 1;                                          // [tiles] scores written (and the P V before them done)
-    uint64_t* p_full = s_full + kTiles;                                     // [tiles] P written
-    uint64_t* o_full = p_full + kTiles;                                     // [tiles] the last P V done
-    uint64_t* drained = o_full + kTiles;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+    uint64_t* p_full = s_full + kTiles;                                     // [tiles][chunks] P written
+    uint64_t* o_full = p_full + kTiles * S::chunks;                         // [tiles] the last P V done
+    uint64_t* drained = o_full + kTiles;                                    // [tiles]
+    uint64_t* turn = drained + kTiles;                                      // [tiles] the other tile's exponentials done
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     ChBlock* block_s = reinterpret_cast<ChBlock*>(tmem_slot + 2);
 
@@ -118,14 +117,14 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     const int group = p.q_heads / p.kv_heads, tile_tokens = kChRows / group;
     const int split = int(blockIdx.x) % splits, kv = int(blockIdx.x) / splits % p.kv_heads, y = int(blockIdx.x) / splits / p.kv_heads;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], S::loaders), mbar_init(&empty[s], kTiles);
         mbar_init(q_full, 1);
-        for (int q = 0; q < kTiles; ++q) mbar_init(&s_full[q], 1), mbar_init(&p_full[q], 4), mbar_init(&o_full[q], 1);
-        mbar_init(drained, 1);
+        for (int q = 0; q < kTiles; ++q) mbar_init(&s_full[q], 1), mbar_init(&o_full[q], 1), mbar_init(&drained[q], 1), mbar_init(&turn[q], 4);
+        for (int c = 0; c < kTiles * S::chunks; ++c) mbar_init(&p_full[c], 4);
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == S::mma_warp) {
+    if (warp == S::load_warp) {
         tmem_alloc(tmem_slot, S::cols);
         tmem_relinquish();
     }
@@ -141,7 +140,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const ChBlock blk = *block_s;
     if (blk.b < 0) {   // no rows for this CTA, and none for the others of its cluster
-        if (warp == S::mma_warp) tmem_dealloc(tmem_base, S::cols);
+        if (warp == S::load_warp) tmem_dealloc(tmem_base, S::cols);
         return;
     }
     // keys that a tile's last row sees, and the steps of this CTA
@@ -161,141 +160,155 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
         most_steps = max(most_steps, steps[q]);
     }
 
-    if (warp == S::load_warp) {
-        // ---------------------------------------------------------------- loader
+    if (warp >= S::load_warp) {
+        // --------------------------------------------------------------- loaders
+        const int lw = warp - S::load_warp;
         if (most_steps) {
-            if (lane == 0) {
+            if (lw == 0 && elect_one()) {
                 mbar_expect_tx(q_full, kTiles * S::q_tile);
                 for (int q = 0; q < kTiles; ++q)
                     for (int h = 0; h < 2; ++h)
-                        tma_load_2d(smem + S::q + q * S::q_tile + h * S::q_half, &maps.q, h * 64,
+                        tma_load_2d(smem + S::q + q * S::q_tile + h * S::q_half, &q_map, h * 64,
                                     (kv * p.tokens + blk.row0 + blk.first + q * tile_tokens) * group, q_full);
             }
+            __syncwarp();
+            // Rounds of 32 keys go round the loaders; a lane looks up the page of one key of each round.
             const int* table = p.tables + size_t(blk.b) * p.width;
-            const int boxes = kKeys / box, nowhere = p.physical_pages * p.page_size;
-            constexpr int kMost = kKeys / 32;
-            // first cache row of a lane's boxes, `nowhere` for those without a page
-            int at[kMost], next[kMost];
-            const auto look_up = [&](int j, int (&r)[kMost]) {
+            constexpr int kRounds = kKeys / 32, kMine = (kRounds + S::loaders - 1) / S::loaders;
+            int page[kMine], row[kMine], logical[kMine], within[kMine];   // of the step looked up last
+            const int step_pages = kKeys / p.page_size, step_rest = kKeys % p.page_size;
+            const auto look_up = [&](int j) {
 #pragma unroll
-                for (int u = 0; u < kMost; ++u) {
-                    const int i = u * 32 + lane, pos = (step0 + j) * kKeys + i * box;
-                    r[u] = nowhere;
-                    if (i < boxes && j < most_steps && pos < most) {
-                        const int page = table[pos / p.page_size];
-                        if (page >= 0 && page < p.physical_pages) r[u] = page * p.page_size + pos % p.page_size;
+                for (int u = 0; u < kMine; ++u) {
+                    const int round = u * S::loaders + lw, pos = (step0 + j) * kKeys + round * 32 + lane;
+                    if (j == 0) {
+                        logical[u] = pos / p.page_size, within[u] = pos % p.page_size;
+                    } else {
+                        logical[u] += step_pages, within[u] += step_rest;
+                        if (within[u] >= p.page_size) within[u] -= p.page_size, ++logical[u];
                     }
+                    page[u] = round < kRounds && j < most_steps && pos < most ? __ldg(table + logical[u]) : -1;
                 }
             };
-            const auto request = [&](const CUtensorMap* map, const CUtensorMap* row_map, int n, int j) -> bool {
+            const size_t row_bytes = size_t(p.kv_heads) * kChDim * 2;
+            const int piece = lane & 15, upper = lane >> 4;
+            const size_t column = size_t(kv) * kChDim * 2 + piece * 16;
+            uint32_t to_off[4];   // where a lane's 16 bytes of rows 0 and 1, 2 and 3, ... of eight go: the swizzle
+#pragma unroll
+            for (int i = 0; i < 4; ++i) to_off[i] = (piece >> 3) * S::half + (2 * i + upper) * 128 + (((piece & 7) ^ (2 * i + upper)) << 4);
+            // two rows of 256 bytes per copy instruction; rows that do not exist are filled with zeros
+            const auto request = [&](const __nv_bfloat16* cache, int n) -> bool {
                 const int slot = n % kSlots;
                 if (n >= kSlots && !mbar_wait_warp(&empty[slot], ((n / kSlots) - 1) & 1, abort_flag)) return false;
-                if (lane == 0) mbar_expect_tx(&full[slot], S::slot);
-                __syncwarp();
-                uint8_t* to = smem + S::ring + slot * S::slot;
+                const char* from = reinterpret_cast<const char*>(cache) + column;
+                const uint32_t to = smem_u32(smem + S::ring + slot * S::slot);
 #pragma unroll
-                for (int u = 0; u < kMost; ++u) {
-                    const int i = u * 32 + lane, pos = (step0 + j) * kKeys + i * box;
-                    if (i >= boxes) continue;
-                    if (pos + box <= most || pos >= most || at[u] == nowhere) {
-                        tma_load_3d(to + i * box * 128, map, 0, kv, at[u], &full[slot]);
-                        tma_load_3d(to + S::half + i * box * 128, map, 64, kv, at[u], &full[slot]);
-                    } else {
-                        for (int r = 0; r < box; ++r) {
-                            const int from = pos + r < most ? at[u] + r : nowhere;
-                            tma_load_3d(to + (i * box + r) * 128, row_map, 0, kv, from, &full[slot]);
-                            tma_load_3d(to + S::half + (i * box + r) * 128, row_map, 64, kv, from, &full[slot]);
-                        }
-                    }
+                for (int u = 0; u < kMine; ++u) {
+                    const int round = u * S::loaders + lw;
+                    if (round >= kRounds) break;
+                    int r[16];   // all at once: a copy that waits for its own row's number takes 50 clocks
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) r[i] = __shfl_sync(0xffffffffu, row[u], 2 * i + upper);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        cp_async16(to + to_off[i & 3] + (round * 4 + (i >> 2)) * 1024, from + size_t(max(r[i], 0)) * row_bytes, r[i] >= 0);
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
                 return true;
             };
-            look_up(0, at);
-            int n = 0;
-            for (int j = 0; j < most_steps; ++j) {
-                look_up(j + 1, next);
-                // which keys there are: the softmax of step j - 4 has long been done when the ring takes step j
-                uint32_t there[kMost], all = 0xffffffffu;
-#pragma unroll
-                for (int u = 0; u < kMost; ++u) {
-                    there[u] = __ballot_sync(0xffffffffu, u * 32 + lane >= boxes || at[u] != nowhere);
-                    all &= there[u];
-                }
-                if (lane < kKeys / 32) {
-                    uint32_t bits = 0xffffffffu;
-                    if (all != 0xffffffffu) {
-                        bits = 0;
-                        for (int k = 0; k < 32; k += min(box, 32)) {
-                            const int i = (lane * 32 + k) / box;
-                            uint32_t word = 0;
-#pragma unroll
-                            for (int u = 0; u < kMost; ++u) word = (i >> 5) == u ? there[u] : word;
-                            if ((word >> (i & 31)) & 1) bits |= (box >= 32 ? 0xffffffffu : (1u << box) - 1u) << k;
-                        }
-                    }
-                    exists[(j & 3) * (kKeys / 32) + lane] = bits;
-                }
+            const auto announce = [&](int n) {
+                fence_proxy_async_smem();
                 __syncwarp();
-                if (!request(&maps.k, &maps.k_row, n, j) || !request(&maps.v, &maps.v_row, n + 1, j)) break;
-                n += 2;
+                if (lane == 0) mbar_arrive(&full[n % kSlots]);
+            };
+            look_up(0);
+            int sent = 0;   // requests so far; all but the last two have been announced
+            for (int j = 0; j < most_steps; ++j) {
 #pragma unroll
-                for (int u = 0; u < kMost; ++u) at[u] = next[u];
+                for (int u = 0; u < kMine; ++u) {
+                    const bool there = page[u] >= 0 && page[u] < p.physical_pages;
+                    row[u] = there ? page[u] * p.page_size + within[u] : -1;
+                    const uint32_t bits = __ballot_sync(0xffffffffu, there);
+                    // which keys there are: the softmax of step j - 4 has long been done when the ring takes step j
+                    if (lane == 0 && u * S::loaders + lw < kRounds) exists[(j & 3) * kRounds + u * S::loaders + lw] = bits;
+                }
+                look_up(j + 1);   // asked for a step ahead
+                if (!request(p.keys, 2 * j)) break;
+                if (j > 0) {
+                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    announce(2 * j - 2);
+                }
+                ++sent;
+                if (!request(p.values, 2 * j + 1)) break;
+                if (j > 0) {
+                    asm volatile("cp.async.wait_group 2;" ::: "memory");
+                    announce(2 * j - 1);
+                }
+                ++sent;
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            if (sent == 2 * most_steps) announce(sent - 2), announce(sent - 1);
             // nothing is in flight when the CTA gives its memory back, also after a wait that gave up
-            mbar_wait_suspended(q_full, 0);
-            ring_wait_landed(full, kSlots, uint32_t(n % kSlots), uint32_t(n / kSlots));
+            if (lw == 0) mbar_wait_suspended(q_full, 0);
             __syncwarp();
         }
-    } else if (warp == S::mma_warp) {
-        // ----------------------------------------------------------- MMA issuer
+    } else if (warp >= S::mma_warp) {
+        // ------------------------------------------- MMA issuers, one per tile
         if (most_steps && elect_one()) {
             constexpr uint32_t idesc_qk = umma_idesc_f16(1, kChRows, kKeys);
             constexpr uint32_t idesc_pv = umma_idesc_f16(1, kChRows, kChDim) | (1u << 16);   // V: MN-major
-            const uint32_t q_lo = umma_desc_lo(smem_u32(smem + S::q)), k_lo = umma_desc_lo(smem_u32(smem + S::ring));
+            const int q = warp - S::mma_warp;
+            int my_steps = 0;
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
+            const uint32_t tile = tmem_base + q * S::tile_cols;
+            const uint32_t q_lo = umma_desc_lo(smem_u32(smem + S::q + q * S::q_tile)), k_lo = umma_desc_lo(smem_u32(smem + S::ring));
             const uint32_t v_lo = ((smem_u32(smem + S::ring) & 0x3FFFFu) >> 4) | (uint32_t(S::half >> 4) << 16);   // the halves of 64 dims
-            const auto scores = [&](int q, uint32_t slot) {
-                const uint32_t a = q_lo + q * (S::q_tile >> 4), k = k_lo + slot * (S::slot >> 4);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int k16 = 0; k16 < 4; ++k16)
-                        umma_f16_ss(tmem_base + q * S::tile_cols, a + h * (S::q_half >> 4) + k16 * 2, k + h * (S::half >> 4) + k16 * 2, idesc_qk, h + k16 > 0);
-                umma_commit(&s_full[q]);
-            };
             const auto wait_slot = [&](int n) {
                 const bool ok = mbar_wait_suspended(&full[n % kSlots], (n / kSlots) & 1);
                 tc_fence_after();
                 return ok;
             };
-            bool good = mbar_wait_suspended(q_full, 0) && wait_slot(0);
-            if (good) {
+            // scores of step j; its keys are then free
+            const auto scores = [&](int j) -> bool {
+                if (!wait_slot(2 * j)) return false;
+                const uint32_t k = k_lo + (2 * j % kSlots) * (S::slot >> 4);
 #pragma unroll
-                for (int q = 0; q < kTiles; ++q)
-                    if (steps[q] > 0) scores(q, 0);
-                umma_commit(&empty[0]);
-            }
-            for (int j = 0; j < most_steps && good; ++j) {
-                const int nv = 2 * j + 1, nk = 2 * j + 2;
-                good = wait_slot(nv) && (j + 1 >= most_steps || wait_slot(nk));
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int q = 0; q < kTiles; ++q) {
-                    if (!good || j >= steps[q]) continue;
-                    good = mbar_wait_suspended(&p_full[q], j & 1);
-                    if (!good) continue;
+                    for (int k16 = 0; k16 < 4; ++k16)
+                        umma_f16_ss(tile, q_lo + h * (S::q_half >> 4) + k16 * 2, k + h * (S::half >> 4) + k16 * 2, idesc_qk, h + k16 > 0);
+                umma_commit(&s_full[q]);
+                umma_commit(&empty[2 * j % kSlots]);
+                return true;
+            };
+            bool good = mbar_wait_suspended(q_full, 0) && (my_steps == 0 || scores(0));
+            for (int j = 0; j < my_steps && good; ++j) {
+                const int nv = 2 * j + 1;
+                good = wait_slot(nv);
+                const uint32_t v = v_lo + (nv % kSlots) * (S::slot >> 4);
+#pragma unroll
+                for (int c = 0; c < S::chunks; ++c) {
+                    good = good && mbar_wait_suspended(&p_full[q * S::chunks + c], j & 1);
+                    if (!good) break;
                     tc_fence_after();
-                    const uint32_t tile = tmem_base + q * S::tile_cols, v = v_lo + (nv % kSlots) * (S::slot >> 4);
 #pragma unroll
-                    for (int k16 = 0; k16 < kKeys / 16; ++k16)
+                    for (int k16 = 2 * c; k16 < 2 * c + 2; ++k16)
                         umma_f16_ts(tile + S::col_o, tile + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, j > 0 || k16 > 0);
-                    if (j + 1 < steps[q]) scores(q, nk % kSlots);
-                    else umma_commit(&o_full[q]);
                 }
+                if (!good) break;
                 umma_commit(&empty[nv % kSlots]);
-                if (j + 1 < most_steps) umma_commit(&empty[nk % kSlots]);
+                if (j + 1 < my_steps) good = scores(j + 1);
+                else umma_commit(&o_full[q]);
+            }
+            // the steps that only the other tile has: passed on as they come
+            for (int n = 2 * my_steps; n < 2 * most_steps && good; ++n) {
+                good = wait_slot(n);
+                mbar_arrive(&empty[n % kSlots]);
             }
             if (!good) *abort_flag = 1;
-            umma_commit(drained);   // no MMA is in flight when the CTA gives its memory back, also after a wait that gave up
-            mbar_wait_suspended(drained, 0);
+            umma_commit(&drained[q]);   // no MMA is in flight when the CTA gives its memory back, also after a wait that gave up
+            mbar_wait_suspended(&drained[q], 0);
         }
         __syncwarp();
     } else {
@@ -308,6 +321,9 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
+        // steps in which the tiles take turns with their exponentials: left alone they run in step, both on the exponential unit and
+        // then both on the tensor pipe
+        const int turns = kTiles == 2 ? min(steps[0], steps[kTiles - 1]) : 0;
         constexpr float kScale = 0.08838834764831845f * 1.4426950408889634f;   // 1 / sqrt(128), in powers of two
         float ref = -INFINITY, sum = 0.f;                                      // what the exponents are taken against; the weights' sum
         bool good = true;
@@ -334,12 +350,14 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
                     for (int i = 0; i < 32; ++i) s[c][i] = (vis >> i) & 1 ? s[c][i] : 0xff800000u;   // -inf
                 }
             }
-            float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            float m[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
 #pragma unroll
             for (int c = 0; c < kKeys / 32; ++c)
 #pragma unroll
-                for (int i = 0; i < 32; i += 2) m[(i >> 1) & 3] = max3(m[(i >> 1) & 3], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
-            const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * kScale;
+                for (int i = 0; i < 32; i += 2) m[(i >> 1) & 7] = max3(m[(i >> 1) & 7], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
+            const float top = max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7])) * kScale;
             const bool grow = top > ref + 8.f;
             if (__any_sync(0xffffffffu, grow)) {
                 const float f = grow ? ex2(ref - top) : 1.f;
@@ -364,9 +382,20 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
             }
             const float base = ref == -INFINITY ? 0.f : ref;
             const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base);
+            if (kTiles == 2 && j < turns && (q == 1 || j > 0)) {
+                good = mbar_wait_warp(&turn[q], (j - (q == 0)) & 1, abort_flag);
+                if (!good) break;
+            }
             uint64_t part2[2] = {0, 0};
+            // a chunk is handed over when the next one is computed: its store has had that long
+            const auto hand_over = [&](int c) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[q * S::chunks + c]);
+            };
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) {
+            for (int c = 0; c < S::chunks; ++c) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -376,15 +405,14 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
                     part2[i & 1] = add2(part2[i & 1], f32x2(a, d));
                     w[i] = bf16x2_of(a, d);
                 }
+                if (c) hand_over(c - 1);
                 tmem_st_32x16(tm + 16 * c, w);
             }
+            if (kTiles == 2 && j < turns && lane == 0) mbar_arrive(&turn[1 - q]);   // nobody waits for tile 1's last one
+            hand_over(S::chunks - 1);
             float part[2];
             f32x2_split(add2(part2[0], part2[1]), part[0], part[1]);
             sum += part[0] + part[1];
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[q]);
         }
         if (my_steps && good) good = mbar_wait_warp(&o_full[q], 0, abort_flag);
         tc_fence_after();
@@ -482,38 +510,18 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == S::mma_warp) {
+    if (warp == S::load_warp) {
         tc_fence_after();
         tmem_dealloc(tmem_base, S::cols);
     }
-}
-
-// [physical pages x page size] cache rows of kv_heads x 128, boxes of `rows` rows x 64 dims of one kv head, 128-byte swizzle.
-int cache_map(CUtensorMap* map, const void* base, const Chunk& p, int rows)
-{
-    TensorMapEncodeFn enc = tensor_map_encoder();
-    if (!enc) return fail(GARNET_B200_NOT_SUPPORTED, "cuTensorMapEncodeTiled is not available from this driver");
-    const cuuint64_t dims[3] = {kChDim, cuuint64_t(p.kv_heads), cuuint64_t(p.physical_pages) * p.page_size};
-    const cuuint64_t strides[2] = {kChDim * 2, cuuint64_t(p.kv_heads) * kChDim * 2};
-    const cuuint32_t box[3] = {64, 1, cuuint32_t(rows)}, ones[3] = {1, 1, 1};
-    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(GARNET_B200_CUDA_ERROR, "cuTensorMapEncodeTiled (cache) failed with code %d", int(r));
-    return GARNET_B200_OK;
 }
 
 template <int kTiles, int kKeys, int kSlots>
 int launch(const Chunk& p, int splits, cudaStream_t stream)
 {
     using S = ChShape<kTiles, kKeys, kSlots>;
-    int box = kKeys;   // rows that lie together in every page: the largest power of two that divides the page size, up to a step
-    while (p.page_size % box) box /= 2;
-    ChMaps maps;
-    if (int rc = make_tensor_map_2d_16bit(&maps.q, p.queries, uint64_t(p.tokens) * p.q_heads, kChDim, kChRows)) return rc;
-    if (int rc = cache_map(&maps.k, p.keys, p, box)) return rc;
-    if (int rc = cache_map(&maps.v, p.values, p, box)) return rc;
-    if (int rc = cache_map(&maps.k_row, p.keys, p, 1)) return rc;
-    if (int rc = cache_map(&maps.v_row, p.values, p, 1)) return rc;
+    CUtensorMap q_map;
+    if (int rc = make_tensor_map_2d_16bit(&q_map, p.queries, uint64_t(p.tokens) * p.q_heads, kChDim, kChRows)) return rc;
     const auto kernel = attn_chunk_tc_kernel<kTiles, kKeys, kSlots>;
     GB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total));
     // blocks of a sequence's rows: ceil(rows / block) summed over the sequences, of whose lengths the host knows the sum's limit only
@@ -532,7 +540,7 @@ int launch(const Chunk& p, int splits, cudaStream_t stream)
     attr[1].val.clusterDim = {unsigned(splits), 1, 1};
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    GB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, maps, box, splits));
+    GB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p, q_map, splits));
     return GARNET_B200_OK;
 }
 

@@ -57,10 +57,6 @@ __device__ __forceinline__ void oss_attention_row(const OssAttn& p, int row, int
         p.out[size_t(row) * p.q_heads * p.head_dim + head * p.head_dim + d] = bf16_round_f(accum[i] / sum);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid)
-{
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
 #endif
 
 // gpt_oss_prefill.cu: many query rows of 64-wide heads on the tensor cores.  `oss_prefill_takes` says whether the shape and
