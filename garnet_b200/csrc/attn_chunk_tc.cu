@@ -33,25 +33,36 @@ namespace cg = cooperative_groups;
 
 constexpr int kChRows = 128;      // query rows of a tile (UMMA M, one softmax thread each)
 constexpr int kChMaxSplits = 8;
+constexpr int kKeys = 64;         // keys of a step (UMMA N of Q K^T, K of P V)
+constexpr int kChRounds = kKeys / 32;   // P is handed over, and rows are copied, 32 keys at a time
+constexpr int kChExists = 8;      // steps whose key bits are kept: more than the ring holds
 
-template <int kTiles, int kKeys, int kSlots>
+template <int kTiles, int kUnits>
 struct ChShape {
     // warps are allocated four at a time: 12 leave a thread 168 registers, twice 8 leave it 128
     static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, load_warp = mma_warp + kTiles, loaders = 4 - kTiles;
     static constexpr int threads = (load_warp + loaders) * 32;
-    static constexpr int chunks = kKeys / 32;   // P is handed over 32 keys at a time
+    static constexpr int ahead = kUnits > 2 ? 3 : 1;                      // units under way when the next is asked for
     static constexpr int q_half = kChRows * 128, q_tile = 2 * q_half;    // 64 dims of a tile of queries; all of them
-    static constexpr int half = kKeys * 128, slot = 2 * half;            // the same of a step's keys (or values)
-    static constexpr int q = 0, ring = kTiles * q_tile, exists = ring + kSlots * slot, bars = exists + 4 * (kKeys / 32) * 4;
-    static constexpr int total = bars + 256 + 1024;                      // barriers, and slack for 1024-byte alignment
+    static constexpr int half = kKeys * 128, slot = 2 * half, unit = 2 * slot;   // the same of a step's keys (or values); keys and values
+    static constexpr int q = 0, ring = kTiles * q_tile, exists = ring + kUnits * unit, bars = exists + kChExists * kChRounds * 4;
+    static constexpr int total = bars + 512 + 1024;                      // barriers, and slack for 1024-byte alignment
     // partial results of a split call, over the queries and the ring: rows of 128 floats, 16 bytes apart in the banks; maxima, sums
     static constexpr int part_row = (kChDim + 4) * 4, stats = kTiles * kChRows * part_row;
     static_assert(stats + kTiles * kChRows * 8 <= exists, "the partial results fit where the queries and the ring were");
     static_assert(total <= 227 * 1024, "shared memory budget");
-    // tensor memory of a tile: the scores (P replaces them), O
-    static constexpr uint32_t col_o = kKeys, tile_cols = kKeys + kChDim, cols = kTiles * tile_cols <= 256 ? 256 : 512;
+    // tensor memory of a tile: two sets of scores (P replaces them), O
+    static constexpr uint32_t col_o = 2 * kKeys, tile_cols = col_o + kChDim, cols = kTiles * tile_cols;
     static_assert(kTiles * tile_cols <= 512, "tensor memory");
 };
+
+// mbar_wait_warp without suspending: the softmax has its scores a hundred clocks sooner.
+__device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
+{
+    const bool all = __all_sync(0xffffffffu, mbar_wait(bar, parity));
+    if (!all) *abort_flag = 1;
+    return all;
+}
 
 // The query rows of a CTA: up to `rows` tokens of sequence b from its token `first` on.
 struct ChBlock {
@@ -93,23 +104,21 @@ __device__ __forceinline__ ChBlock chunk_block(const Chunk& p, int y, int rows, 
     return ChBlock{-1, 0, 0, 0, 0};
 }
 
-template <int kTiles, int kKeys, int kSlots>
-__global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTiles == 1 ? 2 : 1)
+template <int kTiles, int kUnits>
+__global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 ? 2 : 1)
     attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
 {
-    using S = ChShape<kTiles, kKeys, kSlots>;
+    using S = ChShape<kTiles, kUnits>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint32_t* exists = reinterpret_cast<uint32_t*>(smem + S::exists);       // [4 steps][kKeys / 32]: bits of the keys that have a page
-    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::bars);           // [slots]
-    uint64_t* empty = full + kSlots;                                        // [slots]
-    uint64_t* q_full = empty + kSlots;
-    uint64_t* s_full = q_full + 1;                                          // [tiles] scores written (and the P V before them done)
-    uint64_t* p_full = s_full + kTiles;                                     // [tiles][chunks] P written
-    uint64_t* o_full = p_full + kTiles * S::chunks;                         // [tiles] the last P V done
-    uint64_t* drained = o_full + kTiles;                                    // [tiles]
-    uint64_t* turn = drained + kTiles;                                      // [tiles] the other tile's exponentials done
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + kTiles);
+    uint32_t* exists = reinterpret_cast<uint32_t*>(smem + S::exists);       // [4 steps][kChRounds]: bits of the keys that have a page
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::bars);           // [units]
+    uint64_t* empty = full + kUnits;                                        // [units]
+    uint64_t* q_full = empty + kUnits;
+    uint64_t* s_full = q_full + 1;                                          // [tiles][2 sets] scores written, and P V of two steps before done
+    uint64_t* p_full = s_full + kTiles * 2;                                 // [tiles][2 sets] P written
+    uint64_t* drained = p_full + kTiles * 2;                                // [tiles]
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     ChBlock* block_s = reinterpret_cast<ChBlock*>(tmem_slot + 2);
 
@@ -117,10 +126,10 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     const int group = p.q_heads / p.kv_heads, tile_tokens = kChRows / group;
     const int split = int(blockIdx.x) % splits, kv = int(blockIdx.x) / splits % p.kv_heads, y = int(blockIdx.x) / splits / p.kv_heads;
     if (threadIdx.x == 0) {
-        for (int s = 0; s < kSlots; ++s) mbar_init(&full[s], S::loaders), mbar_init(&empty[s], kTiles);
+        for (int u = 0; u < kUnits; ++u) mbar_init(&full[u], S::loaders), mbar_init(&empty[u], kTiles);
         mbar_init(q_full, 1);
-        for (int q = 0; q < kTiles; ++q) mbar_init(&s_full[q], 1), mbar_init(&o_full[q], 1), mbar_init(&drained[q], 1), mbar_init(&turn[q], 4);
-        for (int c = 0; c < kTiles * S::chunks; ++c) mbar_init(&p_full[c], 4);
+        for (int i = 0; i < kTiles * 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+        for (int q = 0; q < kTiles; ++q) mbar_init(&drained[q], 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -174,7 +183,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
             __syncwarp();
             // Rounds of 32 keys go round the loaders; a lane looks up the page of one key of each round.
             const int* table = p.tables + size_t(blk.b) * p.width;
-            constexpr int kRounds = kKeys / 32, kMine = (kRounds + S::loaders - 1) / S::loaders;
+            constexpr int kMine = (kChRounds + S::loaders - 1) / S::loaders;
             int page[kMine], row[kMine], logical[kMine], within[kMine];   // of the step looked up last
             const int step_pages = kKeys / p.page_size, step_rest = kKeys % p.page_size;
             const auto look_up = [&](int j) {
@@ -187,7 +196,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
                         logical[u] += step_pages, within[u] += step_rest;
                         if (within[u] >= p.page_size) within[u] -= p.page_size, ++logical[u];
                     }
-                    page[u] = round < kRounds && j < most_steps && pos < most ? __ldg(table + logical[u]) : -1;
+                    page[u] = round < kChRounds && j < most_steps && pos < most ? __ldg(table + logical[u]) : -1;
                 }
             };
             const size_t row_bytes = size_t(p.kv_heads) * kChDim * 2;
@@ -197,57 +206,53 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
 #pragma unroll
             for (int i = 0; i < 4; ++i) to_off[i] = (piece >> 3) * S::half + (2 * i + upper) * 128 + (((piece & 7) ^ (2 * i + upper)) << 4);
             // two rows of 256 bytes per copy instruction; rows that do not exist are filled with zeros
-            const auto request = [&](const __nv_bfloat16* cache, int n) -> bool {
-                const int slot = n % kSlots;
-                if (n >= kSlots && !mbar_wait_warp(&empty[slot], ((n / kSlots) - 1) & 1, abort_flag)) return false;
+            const auto copy = [&](const __nv_bfloat16* cache, const int (&rows)[kMine], uint32_t to) {
                 const char* from = reinterpret_cast<const char*>(cache) + column;
-                const uint32_t to = smem_u32(smem + S::ring + slot * S::slot);
 #pragma unroll
                 for (int u = 0; u < kMine; ++u) {
                     const int round = u * S::loaders + lw;
-                    if (round >= kRounds) break;
+                    if (round >= kChRounds) break;
                     int r[16];   // all at once: a copy that waits for its own row's number takes 50 clocks
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) r[i] = __shfl_sync(0xffffffffu, row[u], 2 * i + upper);
+                    for (int i = 0; i < 16; ++i) r[i] = __shfl_sync(0xffffffffu, rows[u], 2 * i + upper);
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         cp_async16(to + to_off[i & 3] + (round * 4 + (i >> 2)) * 1024, from + size_t(max(r[i], 0)) * row_bytes, r[i] >= 0);
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                return true;
             };
-            const auto announce = [&](int n) {
+            const auto announce = [&](int u) {
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[n % kSlots]);
+                if (lane == 0) mbar_arrive(&full[u % kUnits]);
             };
             look_up(0);
-            int sent = 0;   // requests so far; all but the last two have been announced
-            for (int j = 0; j < most_steps; ++j) {
+            int before[kMine], before_that[kMine];   // rows of the last two steps
+#pragma unroll
+            for (int u = 0; u < kMine; ++u) before[u] = before_that[u] = -1;
+            int sent = 0;
+            for (; sent < most_steps + 2; ++sent) {
 #pragma unroll
                 for (int u = 0; u < kMine; ++u) {
                     const bool there = page[u] >= 0 && page[u] < p.physical_pages;
                     row[u] = there ? page[u] * p.page_size + within[u] : -1;
                     const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    // which keys there are: the softmax of step j - 4 has long been done when the ring takes step j
-                    if (lane == 0 && u * S::loaders + lw < kRounds) exists[(j & 3) * kRounds + u * S::loaders + lw] = bits;
+                    // which keys there are: the softmax of eight steps before has long been done when the ring takes this one
+                    if (lane == 0 && u * S::loaders + lw < kChRounds) exists[(sent % kChExists) * kChRounds + u * S::loaders + lw] = bits;
                 }
-                look_up(j + 1);   // asked for a step ahead
-                if (!request(p.keys, 2 * j)) break;
-                if (j > 0) {
-                    asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    announce(2 * j - 2);
-                }
-                ++sent;
-                if (!request(p.values, 2 * j + 1)) break;
-                if (j > 0) {
-                    asm volatile("cp.async.wait_group 2;" ::: "memory");
-                    announce(2 * j - 1);
-                }
-                ++sent;
+                look_up(sent + 1);   // asked for a step ahead
+                if (sent >= kUnits && !mbar_wait_warp(&empty[sent % kUnits], ((sent / kUnits) - 1) & 1, abort_flag)) break;
+                const uint32_t to = smem_u32(smem + S::ring + sent % kUnits * S::unit);
+                if (sent < most_steps) copy(p.keys, row, to);
+                if (sent >= 2) copy(p.values, before_that, to + S::slot);
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group %0;" ::"n"(S::ahead) : "memory");
+                if (sent >= S::ahead) announce(sent - S::ahead);
+#pragma unroll
+                for (int u = 0; u < kMine; ++u) before_that[u] = before[u], before[u] = row[u];
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
-            if (sent == 2 * most_steps) announce(sent - 2), announce(sent - 1);
+            if (sent == most_steps + 2)
+                for (int u = max(0, sent - S::ahead); u < sent; ++u) announce(u);
             // nothing is in flight when the CTA gives its memory back, also after a wait that gave up
             if (lw == 0) mbar_wait_suspended(q_full, 0);
             __syncwarp();
@@ -263,48 +268,36 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
             for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
             const uint32_t tile = tmem_base + q * S::tile_cols;
             const uint32_t q_lo = umma_desc_lo(smem_u32(smem + S::q + q * S::q_tile)), k_lo = umma_desc_lo(smem_u32(smem + S::ring));
-            const uint32_t v_lo = ((smem_u32(smem + S::ring) & 0x3FFFFu) >> 4) | (uint32_t(S::half >> 4) << 16);   // the halves of 64 dims
-            const auto wait_slot = [&](int n) {
-                const bool ok = mbar_wait_suspended(&full[n % kSlots], (n / kSlots) & 1);
-                tc_fence_after();
-                return ok;
-            };
-            // scores of step j; its keys are then free
-            const auto scores = [&](int j) -> bool {
-                if (!wait_slot(2 * j)) return false;
-                const uint32_t k = k_lo + (2 * j % kSlots) * (S::slot >> 4);
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int k16 = 0; k16 < 4; ++k16)
-                        umma_f16_ss(tile, q_lo + h * (S::q_half >> 4) + k16 * 2, k + h * (S::half >> 4) + k16 * 2, idesc_qk, h + k16 > 0);
-                umma_commit(&s_full[q]);
-                umma_commit(&empty[2 * j % kSlots]);
-                return true;
-            };
-            bool good = mbar_wait_suspended(q_full, 0) && (my_steps == 0 || scores(0));
-            for (int j = 0; j < my_steps && good; ++j) {
-                const int nv = 2 * j + 1;
-                good = wait_slot(nv);
-                const uint32_t v = v_lo + (nv % kSlots) * (S::slot >> 4);
-#pragma unroll
-                for (int c = 0; c < S::chunks; ++c) {
-                    good = good && mbar_wait_suspended(&p_full[q * S::chunks + c], j & 1);
+            const uint32_t v_lo = ((smem_u32(smem + S::ring + S::slot) & 0x3FFFFu) >> 4) | (uint32_t(S::half >> 4) << 16);   // the halves of 64 dims
+            // Unit u brings the keys of step u and the values of step u - 2: P V of that one, then the scores of step u into the set
+            // that its P leaves.  Two waits and two commits per step: each costs this thread some 200 clocks beside busy warps.
+            bool good = mbar_wait_suspended(q_full, 0);
+            uint32_t unit = 0, parity = 0;
+            for (int u = 0; u < most_steps + 2 && good; ++u) {
+                const uint32_t set = (u & 1) * kKeys;
+                good = mbar_wait(&full[unit], parity);
+                if (u >= 2 && u < my_steps + 2) {
+                    good = good && mbar_wait(&p_full[q * 2 + (u & 1)], ((u - 2) >> 1) & 1);
                     if (!good) break;
                     tc_fence_after();
+                    const uint32_t v = v_lo + unit * (S::unit >> 4);
 #pragma unroll
-                    for (int k16 = 2 * c; k16 < 2 * c + 2; ++k16)
-                        umma_f16_ts(tile + S::col_o, tile + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, j > 0 || k16 > 0);
+                    for (int k16 = 0; k16 < kKeys / 16; ++k16)
+                        umma_f16_ts(tile + S::col_o, tile + set + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, u > 2 || k16 > 0);
                 }
                 if (!good) break;
-                umma_commit(&empty[nv % kSlots]);
-                if (j + 1 < my_steps) good = scores(j + 1);
-                else umma_commit(&o_full[q]);
-            }
-            // the steps that only the other tile has: passed on as they come
-            for (int n = 2 * my_steps; n < 2 * most_steps && good; ++n) {
-                good = wait_slot(n);
-                mbar_arrive(&empty[n % kSlots]);
+                tc_fence_after();
+                if (u < my_steps) {
+                    const uint32_t k = k_lo + unit * (S::unit >> 4);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k16 = 0; k16 < 4; ++k16)
+                            umma_f16_ss(tile + set, q_lo + h * (S::q_half >> 4) + k16 * 2, k + h * (S::half >> 4) + k16 * 2, idesc_qk, h + k16 > 0);
+                }
+                if (u < my_steps + 2) umma_commit(&s_full[q * 2 + (u & 1)]);
+                umma_commit(&empty[unit]);
+                if (++unit == kUnits) unit = 0, parity ^= 1;
             }
             if (!good) *abort_flag = 1;
             umma_commit(&drained[q]);   // no MMA is in flight when the CTA gives its memory back, also after a wait that gave up
@@ -321,30 +314,30 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
-        // steps in which the tiles take turns with their exponentials: left alone they run in step, both on the exponential unit and
-        // then both on the tensor pipe
-        const int turns = kTiles == 2 ? min(steps[0], steps[kTiles - 1]) : 0;
+        // The scores of step i, and with them P V of step i - 2; behind the last steps that alone.
+        const auto scores_of = [&](int i) { return wait_warp(&s_full[q * 2 + (i & 1)], (i >> 1) & 1, abort_flag); };
         constexpr float kScale = 0.08838834764831845f * 1.4426950408889634f;   // 1 / sqrt(128), in powers of two
         float ref = -INFINITY, sum = 0.f;                                      // what the exponents are taken against; the weights' sum
         bool good = true;
         for (int j = 0; j < my_steps; ++j) {
             const int kb = (step0 + j) * kKeys;
-            good = mbar_wait_warp(&s_full[q], j & 1, abort_flag);
+            const uint32_t ts = tm + (j & 1) * kKeys;
+            good = scores_of(j);
             if (!good) break;
             tc_fence_after();
-            uint32_t s[kKeys / 32][32];
+            uint32_t s[kChRounds][32];
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) tmem_ld_32x32(tm + 32 * c, s[c]);
-            uint32_t there[kKeys / 32], all = 0xffffffffu;
+            for (int c = 0; c < kChRounds; ++c) tmem_ld_32x32(ts + 32 * c, s[c]);
+            uint32_t there[kChRounds], all = 0xffffffffu;
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c) {
-                there[c] = exists[(j & 3) * (kKeys / 32) + c];
+            for (int c = 0; c < kChRounds; ++c) {
+                there[c] = exists[(j % kChExists) * kChRounds + c];
                 all &= there[c];
             }
             tmem_ld_wait();
             if (!__all_sync(0xffffffffu, end >= kb + kKeys && all == 0xffffffffu)) {
 #pragma unroll
-                for (int c = 0; c < kKeys / 32; ++c) {
+                for (int c = 0; c < kChRounds; ++c) {
                     const uint32_t vis = there[c] & bit_range(0, end - kb - 32 * c);
 #pragma unroll
                     for (int i = 0; i < 32; ++i) s[c][i] = (vis >> i) & 1 ? s[c][i] : 0xff800000u;   // -inf
@@ -354,7 +347,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
 #pragma unroll
             for (int i = 0; i < 8; ++i) m[i] = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < kKeys / 32; ++c)
+            for (int c = 0; c < kChRounds; ++c)
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) m[(i >> 1) & 7] = max3(m[(i >> 1) & 7], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
             const float top = max3(max3(m[0], m[1], m[2]), max3(m[3], m[4], m[5]), fmaxf(m[6], m[7])) * kScale;
@@ -363,7 +356,10 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
                 const float f = grow ? ex2(ref - top) : 1.f;
                 if (grow) ref = top;
                 sum *= f;
-                if (j > 0) {   // the P V of the step before is done: its commit came before that of these scores
+                if (j > 0) {
+                    good = scores_of(j + 1);   // O then holds the steps up to the one before this
+                    if (!good) break;
+                    tc_fence_after();
                     const uint64_t f2 = f32x2(f, f);
 #pragma unroll 1
                     for (int c = 0; c < kChDim / 16; ++c) {
@@ -382,20 +378,9 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
             }
             const float base = ref == -INFINITY ? 0.f : ref;
             const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base);
-            if (kTiles == 2 && j < turns && (q == 1 || j > 0)) {
-                good = mbar_wait_warp(&turn[q], (j - (q == 0)) & 1, abort_flag);
-                if (!good) break;
-            }
             uint64_t part2[2] = {0, 0};
-            // a chunk is handed over when the next one is computed: its store has had that long
-            const auto hand_over = [&](int c) {
-                tmem_st_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[q * S::chunks + c]);
-            };
 #pragma unroll
-            for (int c = 0; c < S::chunks; ++c) {
+            for (int c = 0; c < kChRounds; ++c) {
                 uint32_t w[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -405,16 +390,17 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
                     part2[i & 1] = add2(part2[i & 1], f32x2(a, d));
                     w[i] = bf16x2_of(a, d);
                 }
-                if (c) hand_over(c - 1);
-                tmem_st_32x16(tm + 16 * c, w);
+                tmem_st_32x16(ts + 16 * c, w);
             }
-            if (kTiles == 2 && j < turns && lane == 0) mbar_arrive(&turn[1 - q]);   // nobody waits for tile 1's last one
-            hand_over(S::chunks - 1);
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[q * 2 + (j & 1)]);
             float part[2];
             f32x2_split(add2(part2[0], part2[1]), part[0], part[1]);
             sum += part[0] + part[1];
         }
-        if (my_steps && good) good = mbar_wait_warp(&o_full[q], 0, abort_flag);
+        if (my_steps && good) good = scores_of(my_steps + 1);
         tc_fence_after();
         // a wait that gave up leaves NaNs, which no caller can take for a result
         if (!good) sum = NAN;
@@ -516,13 +502,13 @@ __global__ void __launch_bounds__(ChShape<kTiles, kKeys, kSlots>::threads, kTile
     }
 }
 
-template <int kTiles, int kKeys, int kSlots>
+template <int kTiles, int kUnits>
 int launch(const Chunk& p, int splits, cudaStream_t stream)
 {
-    using S = ChShape<kTiles, kKeys, kSlots>;
+    using S = ChShape<kTiles, kUnits>;
     CUtensorMap q_map;
     if (int rc = make_tensor_map_2d_16bit(&q_map, p.queries, uint64_t(p.tokens) * p.q_heads, kChDim, kChRows)) return rc;
-    const auto kernel = attn_chunk_tc_kernel<kTiles, kKeys, kSlots>;
+    const auto kernel = attn_chunk_tc_kernel<kTiles, kUnits>;
     GB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total));
     // blocks of a sequence's rows: ceil(rows / block) summed over the sequences, of whose lengths the host knows the sum's limit only
     const int rows = kChRows / (p.q_heads / p.kv_heads) * kTiles;
@@ -549,7 +535,7 @@ int launch(const Chunk& p, int splits, cudaStream_t stream)
 int chunk_attention_launch(const Chunk& p, cudaStream_t stream)
 {
     const ChunkPlan plan = chunk_plan(p.batch, p.kv_heads, p.tokens, kChRows / (p.q_heads / p.kv_heads), p.max_context);
-    return plan.tiles == 2 ? launch<2, 128, 5>(p, plan.splits, stream) : launch<1, 64, 4>(p, plan.splits, stream);
+    return plan.tiles == 2 ? launch<2, 5>(p, plan.splits, stream) : launch<1, 2>(p, plan.splits, stream);
 }
 
 }  // namespace gb200
