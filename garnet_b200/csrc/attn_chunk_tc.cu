@@ -33,14 +33,20 @@ namespace cg = cooperative_groups;
 
 constexpr int kChRows = 128;      // query rows of a tile (UMMA M, one softmax thread each)
 constexpr int kChMaxSplits = 8;
+// Named barriers between the warps of a tile: a barrier in shared memory takes its waiter 200 clocks beside warps that keep the
+// exponential unit busy, also when it is there already; a named one 30.  Every warp comes to all of its barriers, also after a wait
+// that gave up.
+constexpr int kBarTurn = 1, kBarScores = 3, kBarP = 7;
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int kKeys = 64;         // keys of a step (UMMA N of Q K^T, K of P V)
 constexpr int kChRounds = kKeys / 32;   // P is handed over, and rows are copied, 32 keys at a time
 constexpr int kChExists = 8;      // steps whose key bits are kept: more than the ring holds
 
 template <int kTiles, int kUnits>
 struct ChShape {
-    // warps are allocated four at a time: 12 leave a thread 168 registers, twice 8 leave it 128
-    static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, load_warp = mma_warp + kTiles, loaders = 4 - kTiles;
+    // warps are allocated four at a time: 14, as well as twice 8, leave a thread 128 registers
+    static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, scout_warp = mma_warp + kTiles, load_warp = scout_warp + kTiles, loaders = 2;
     static constexpr int threads = (load_warp + loaders) * 32;
     static constexpr int ahead = kUnits > 2 ? 3 : 1;                      // units under way when the next is asked for
     static constexpr int q_half = kChRows * 128, q_tile = 2 * q_half;    // 64 dims of a tile of queries; all of them
@@ -116,8 +122,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
     uint64_t* empty = full + kUnits;                                        // [units]
     uint64_t* q_full = empty + kUnits;
     uint64_t* s_full = q_full + 1;                                          // [tiles][2 sets] scores written, and P V of two steps before done
-    uint64_t* p_full = s_full + kTiles * 2;                                 // [tiles][2 sets] P written
-    uint64_t* drained = p_full + kTiles * 2;                                // [tiles]
+    uint64_t* drained = s_full + kTiles * 2;                                // [tiles]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     ChBlock* block_s = reinterpret_cast<ChBlock*>(tmem_slot + 2);
@@ -128,7 +133,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
     if (threadIdx.x == 0) {
         for (int u = 0; u < kUnits; ++u) mbar_init(&full[u], S::loaders), mbar_init(&empty[u], kTiles);
         mbar_init(q_full, 1);
-        for (int i = 0; i < kTiles * 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4);
+        for (int i = 0; i < kTiles * 2; ++i) mbar_init(&s_full[i], 1);
         for (int q = 0; q < kTiles; ++q) mbar_init(&drained[q], 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -257,36 +262,47 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
             if (lw == 0) mbar_wait_suspended(q_full, 0);
             __syncwarp();
         }
+    } else if (warp >= S::scout_warp) {
+        // -------------- scouts, one per tile: pass on that scores (and P V of two steps before) are done
+        const int q = warp - S::scout_warp;
+        int my_steps = 0;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
+        bool good = true;
+        for (int i = 0; my_steps && i < my_steps + 2; ++i) {
+            good = good && wait_warp(&s_full[q * 2 + (i & 1)], (i >> 1) & 1, abort_flag);
+            tc_fence_after();
+            tc_fence_before();
+            bar_arrive(kBarScores + q * 2 + (i & 1), 160);
+        }
     } else if (warp >= S::mma_warp) {
         // ------------------------------------------- MMA issuers, one per tile
-        if (most_steps && elect_one()) {
-            constexpr uint32_t idesc_qk = umma_idesc_f16(1, kChRows, kKeys);
-            constexpr uint32_t idesc_pv = umma_idesc_f16(1, kChRows, kChDim) | (1u << 16);   // V: MN-major
-            const int q = warp - S::mma_warp;
-            int my_steps = 0;
+        constexpr uint32_t idesc_qk = umma_idesc_f16(1, kChRows, kKeys);
+        constexpr uint32_t idesc_pv = umma_idesc_f16(1, kChRows, kChDim) | (1u << 16);   // V: MN-major
+        const int q = warp - S::mma_warp;
+        int my_steps = 0;
 #pragma unroll
-            for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
-            const uint32_t tile = tmem_base + q * S::tile_cols;
-            const uint32_t q_lo = umma_desc_lo(smem_u32(smem + S::q + q * S::q_tile)), k_lo = umma_desc_lo(smem_u32(smem + S::ring));
-            const uint32_t v_lo = ((smem_u32(smem + S::ring + S::slot) & 0x3FFFFu) >> 4) | (uint32_t(S::half >> 4) << 16);   // the halves of 64 dims
-            // Unit u brings the keys of step u and the values of step u - 2: P V of that one, then the scores of step u into the set
-            // that its P leaves.  Two waits and two commits per step: each costs this thread some 200 clocks beside busy warps.
-            bool good = mbar_wait_suspended(q_full, 0);
-            uint32_t unit = 0, parity = 0;
-            for (int u = 0; u < most_steps + 2 && good; ++u) {
-                const uint32_t set = (u & 1) * kKeys;
-                good = mbar_wait(&full[unit], parity);
-                if (u >= 2 && u < my_steps + 2) {
-                    good = good && mbar_wait(&p_full[q * 2 + (u & 1)], ((u - 2) >> 1) & 1);
-                    if (!good) break;
-                    tc_fence_after();
+        for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
+        const uint32_t tile = tmem_base + q * S::tile_cols;
+        const uint32_t q_lo = umma_desc_lo(smem_u32(smem + S::q + q * S::q_tile)), k_lo = umma_desc_lo(smem_u32(smem + S::ring));
+        const uint32_t v_lo = ((smem_u32(smem + S::ring + S::slot) & 0x3FFFFu) >> 4) | (uint32_t(S::half >> 4) << 16);   // the halves of 64 dims
+        // Unit u brings the keys of step u and the values of step u - 2: P V of that one, then the scores of step u into the set
+        // that its P leaves.
+        bool good = most_steps == 0 || mbar_wait_warp(q_full, 0, abort_flag);
+        uint32_t unit = 0, parity = 0;
+        for (int u = 0; most_steps && u < most_steps + 2; ++u) {
+            const uint32_t set = (u & 1) * kKeys;
+            good = good && wait_warp(&full[unit], parity, abort_flag);
+            const bool pv = u >= 2 && u < my_steps + 2;
+            if (pv) bar_sync(kBarP + q * 2 + (u & 1), 160);
+            if (good && elect_one()) {
+                tc_fence_after();
+                if (pv) {
                     const uint32_t v = v_lo + unit * (S::unit >> 4);
 #pragma unroll
                     for (int k16 = 0; k16 < kKeys / 16; ++k16)
                         umma_f16_ts(tile + S::col_o, tile + set + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, u > 2 || k16 > 0);
                 }
-                if (!good) break;
-                tc_fence_after();
                 if (u < my_steps) {
                     const uint32_t k = k_lo + unit * (S::unit >> 4);
 #pragma unroll
@@ -297,9 +313,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
                 }
                 if (u < my_steps + 2) umma_commit(&s_full[q * 2 + (u & 1)]);
                 umma_commit(&empty[unit]);
-                if (++unit == kUnits) unit = 0, parity ^= 1;
             }
-            if (!good) *abort_flag = 1;
+            __syncwarp();
+            if (++unit == kUnits) unit = 0, parity ^= 1;
+        }
+        if (most_steps && elect_one()) {
             umma_commit(&drained[q]);   // no MMA is in flight when the CTA gives its memory back, also after a wait that gave up
             mbar_wait_suspended(&drained[q], 0);
         }
@@ -314,16 +332,17 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
-        // The scores of step i, and with them P V of step i - 2; behind the last steps that alone.
-        const auto scores_of = [&](int i) { return wait_warp(&s_full[q * 2 + (i & 1)], (i >> 1) & 1, abort_flag); };
+        // the scores of step i, and with them P V of step i - 2; behind the last steps that alone
+        const auto scores_of = [&](int i) { bar_sync(kBarScores + q * 2 + (i & 1), 160); };
         constexpr float kScale = 0.08838834764831845f * 1.4426950408889634f;   // 1 / sqrt(128), in powers of two
         float ref = -INFINITY, sum = 0.f;                                      // what the exponents are taken against; the weights' sum
-        bool good = true;
+        // steps in which the tiles take turns with their exponentials: left alone they fall into step, first both on the exponential
+        // unit, then neither
+        const int turns = kTiles == 2 ? min(steps[0], steps[kTiles - 1]) : 0;
         for (int j = 0; j < my_steps; ++j) {
             const int kb = (step0 + j) * kKeys;
             const uint32_t ts = tm + (j & 1) * kKeys;
-            good = scores_of(j);
-            if (!good) break;
+            scores_of(j);
             tc_fence_after();
             uint32_t s[kChRounds][32];
 #pragma unroll
@@ -357,8 +376,9 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
                 if (grow) ref = top;
                 sum *= f;
                 if (j > 0) {
-                    good = scores_of(j + 1);   // O then holds the steps up to the one before this
-                    if (!good) break;
+                    // O holds the steps up to the one before this when the next scores are there
+                    if (!*abort_flag) wait_warp(&s_full[q * 2 + ((j + 1) & 1)], ((j + 1) >> 1) & 1, abort_flag);
+                    __syncwarp();
                     tc_fence_after();
                     const uint64_t f2 = f32x2(f, f);
 #pragma unroll 1
@@ -379,6 +399,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
             const float base = ref == -INFINITY ? 0.f : ref;
             const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base);
             uint64_t part2[2] = {0, 0};
+            if (j < turns && (q == 1 || j > 0)) bar_sync(kBarTurn + q, 256);
 #pragma unroll
             for (int c = 0; c < kChRounds; ++c) {
                 uint32_t w[16];
@@ -392,17 +413,18 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
                 }
                 tmem_st_32x16(ts + 16 * c, w);
             }
+            if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
             tmem_st_wait();
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[q * 2 + (j & 1)]);
+            bar_arrive(kBarP + q * 2 + (j & 1), 160);
             float part[2];
             f32x2_split(add2(part2[0], part2[1]), part[0], part[1]);
             sum += part[0] + part[1];
         }
-        if (my_steps && good) good = scores_of(my_steps + 1);
+        if (my_steps) scores_of(my_steps), scores_of(my_steps + 1);
         tc_fence_after();
         // a wait that gave up leaves NaNs, which no caller can take for a result
+        const bool good = !*abort_flag;
         if (!good) sum = NAN;
         if (splits == 1) {
             const float inv = end == 0 || sum == 0.f ? 0.f : 1.f / sum;
