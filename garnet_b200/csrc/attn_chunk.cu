@@ -19,60 +19,96 @@ __device__ __forceinline__ float turned(float a, float cosine, float b, float si
     const float p = __fmul_rn(b, sine);
     return __fadd_rn(__fmaf_rn(a, cosine, p), __fmaf_rn(b, sine, -p));
 }
-__device__ __forceinline__ void unpack(__nv_bfloat162 v, float& a, float& b)
+__device__ __forceinline__ void unpack(const uint4& v, float* x)
 {
-    const float2 f = __bfloat1622float2(v);
-    a = f.x, b = f.y;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
 }
+__device__ __forceinline__ uint4 pack(const float* x) { return make_uint4(bf16x2_of(x[0], x[1]), bf16x2_of(x[2], x[3]), bf16x2_of(x[4], x[5]), bf16x2_of(x[6], x[7])); }
 
-// One CTA per row, a warp per head: a lane holds dims 2 lane, 2 lane + 1 and the two 64 further on, which RoPE turns together.
-// Rounded to bf16 after the norm and after the rotation, as a bf16 network does; the fp32 steps in between carry what
-// their products and the root are short of, and the sum of squares is exact in double: some 1 of 10^6 results is the other bf16
-// neighbour of the float64 result (10 to 20 of 10^6 by plain fp32 steps).
-__global__ void __launch_bounds__(256) attn_chunk_rows_kernel(const Chunk p)
+// A warp takes four heads of a row, eight lanes each: dims 8 l .. 8 l + 7 and the eight 64 further on, which RoPE turns together.
+// Rounded to bf16 after the norm and after the rotation, as a bf16 network does; the fp32 steps in between carry what the sum of
+// squares, the products and the root are short of: some 1 of 10^6 results is the other bf16 neighbour of the float64 result (10 to
+// 20 of 10^6 by plain fp32 steps).
+// Bound: HBM, the rows in and q, k and v out.  8192 rows of 16 / 8 heads: 60 us with a CTA per row, a warp per head and the sums in
+// double.
+constexpr int kRowThreads = 256;
+__global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const Chunk p, const int early)
 {
-    pdl_launch_dependents();
+    // few rows: the attention's CTAs come up beside these; many: they would only take their place
+    if (early) pdl_launch_dependents();
     pdl_wait();
-    const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int b = chunk_sequence(p, row);
-    if (b < 0) return;
-    const int slot = chunk_slot(p, b, row);
-    if (slot < 0) return;
-    const int heads = p.q_heads + 2 * p.kv_heads, group = p.q_heads / p.kv_heads;
-    const float2 cs = reinterpret_cast<const float2*>(p.rope_cos + size_t(slot) * (kChDim / 2))[lane];
-    const float2 sn = reinterpret_cast<const float2*>(p.rope_sin + size_t(slot) * (kChDim / 2))[lane];
-    for (int h = warp; h < heads; h += 8) {
-        const __nv_bfloat162* from = reinterpret_cast<const __nv_bfloat162*>(p.qkv + (size_t(row) * heads + h) * kChDim);
-        __nv_bfloat162 lo = from[lane], hi = from[lane + 32];
-        __nv_bfloat162* to;
-        if (h < p.q_heads) {
-            to = reinterpret_cast<__nv_bfloat162*>(p.queries + ((size_t(h / group) * p.tokens + row) * group + h % group) * kChDim);
-        } else {
-            const long long at = chunk_cache_offset(p, b, slot, (h - p.q_heads) % p.kv_heads);
-            if (at < 0) continue;
-            to = reinterpret_cast<__nv_bfloat162*>((h < p.q_heads + p.kv_heads ? p.keys : p.values) + at);
-        }
-        if (h < p.q_heads + p.kv_heads) {
-            const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(h < p.q_heads ? p.q_norm_w : p.k_norm_w);
-            float x[4], wt[4];
-            unpack(lo, x[0], x[1]), unpack(hi, x[2], x[3]);
-            unpack(w[lane], wt[0], wt[1]), unpack(w[lane + 32], wt[2], wt[3]);
-            double mean = double(x[0] * x[0]) + double(x[1] * x[1]) + double(x[2] * x[2]) + double(x[3] * x[3]);   // exact
-#pragma unroll
-            for (int off = 16; off; off >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, off);
-            mean = mean / kChDim + p.eps;
-            const float r = 1.f / sqrtf(float(mean));
-            const float c = 0.5f * r * float(__fma_rn(-mean, double(r) * r, 1.0));   // what r is short of 1 / sqrt(mean)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float v = __fmul_rn(x[i], wt[i]);   // exact: two bf16 numbers
-                x[i] = bf16_round_f(__fmaf_rn(v, r, __fmul_rn(v, c)));
-            }
-            lo = __floats2bfloat162_rn(turned(x[0], cs.x, -x[2], sn.x), turned(x[1], cs.y, -x[3], sn.y));
-            hi = __floats2bfloat162_rn(turned(x[2], cs.x, x[0], sn.x), turned(x[3], cs.y, x[1], sn.y));
-        }
-        to[lane] = lo, to[lane + 32] = hi;
+    const int lane = threadIdx.x & 31, l = lane & 7, heads = p.q_heads + 2 * p.kv_heads, quads = (heads + 3) / 4, group = p.q_heads / p.kv_heads;
+    const long long task = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+    const int row = int(task / quads), h = int(task % quads) * 4 + (lane >> 3);
+    if (row >= p.tokens) return;
+    const bool has = h < heads, is_q = h < p.q_heads, turns = h < p.q_heads + p.kv_heads;
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo, wlo = lo, whi = lo;
+    if (has) {
+        const uint4* from = reinterpret_cast<const uint4*>(p.qkv + (size_t(row) * heads + h) * kChDim);
+        lo = __ldg(from + l), hi = __ldg(from + 8 + l);
     }
+    if (turns) {
+        const uint4* w = reinterpret_cast<const uint4*>(is_q ? p.q_norm_w : p.k_norm_w);
+        wlo = __ldg(w + l), whi = __ldg(w + 8 + l);
+    }
+    const int b = chunk_sequence(p, row);
+    const int slot = b < 0 ? -1 : chunk_slot(p, b, row);
+    if (slot < 0) return;   // the whole warp
+    float4 cs[2], sn[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        cs[i] = __ldg(reinterpret_cast<const float4*>(p.rope_cos + size_t(slot) * (kChDim / 2)) + 2 * l + i);
+        sn[i] = __ldg(reinterpret_cast<const float4*>(p.rope_sin + size_t(slot) * (kChDim / 2)) + 2 * l + i);
+    }
+    uint4* to = nullptr;
+    if (is_q) {
+        to = reinterpret_cast<uint4*>(p.queries + ((size_t(h / group) * p.tokens + row) * group + h % group) * kChDim);
+    } else if (has) {
+        const long long at = chunk_cache_offset(p, b, slot, (h - p.q_heads) % p.kv_heads);
+        if (at >= 0) to = reinterpret_cast<uint4*>((turns ? p.keys : p.values) + at);
+    }
+    if (__any_sync(0xffffffffu, turns)) {
+        float x[16], w[16];
+        unpack(lo, x), unpack(hi, x + 8), unpack(wlo, w), unpack(whi, w + 8);
+        float sum = 0.f, rest = 0.f;   // the sum of squares and what it is short of
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float next = __fmaf_rn(x[i], x[i], sum);
+            rest = __fadd_rn(rest, __fmaf_rn(x[i], x[i], -__fsub_rn(next, sum)));
+            sum = next;
+        }
+#pragma unroll
+        for (int off = 4; off; off >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, sum, off), a = fmaxf(sum, other), c = fminf(sum, other);
+            rest += __shfl_xor_sync(0xffffffffu, rest, off);
+            sum = __fadd_rn(a, c);
+            rest = __fadd_rn(rest, __fsub_rn(c, __fsub_rn(sum, a)));
+        }
+        const float high = sum * (1.f / kChDim), low = __fmaf_rn(rest, 1.f / kChDim, p.eps), mean = __fadd_rn(high, low);
+        const float short_of = __fsub_rn(low, __fsub_rn(mean, high));
+        const float r = 1.f / sqrtf(mean), square = __fmul_rn(mean, r);
+        // what r is short of 1 / sqrt(mean)
+        const float c = 0.5f * r * (__fmaf_rn(-square, r, 1.f) - __fmaf_rn(mean, r, -square) * r - short_of * r * r);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float v = __fmul_rn(x[i], w[i]);   // exact: two bf16 numbers
+            x[i] = bf16_round_f(__fmaf_rn(v, r, __fmul_rn(v, c)));
+        }
+        if (turns) {
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float cosine = reinterpret_cast<const float*>(cs)[i], sine = reinterpret_cast<const float*>(sn)[i];
+                y[i] = turned(x[i], cosine, -x[i + 8], sine);
+                y[i + 8] = turned(x[i + 8], cosine, x[i], sine);
+            }
+            lo = pack(y), hi = pack(y + 8);
+        }
+    }
+    if (to) to[l] = lo, to[8 + l] = hi;
+    if (!early) pdl_launch_dependents();
 }
 
 int validate_chunk(const garnet_b200_attention_options* o)
@@ -92,20 +128,6 @@ int validate_chunk(const garnet_b200_attention_options* o)
 }
 
 size_t chunk_workspace(const garnet_b200_attention_options& o, int tokens) { return size_t(tokens) * o.q_heads * kChDim * 2; }
-
-cudaError_t chunk_launch(void (*kernel)(Chunk), dim3 grid, cudaStream_t stream, bool dependent, const Chunk& p)
-{
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = dependent ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
-}
 
 }  // namespace
 
@@ -137,10 +159,9 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
         return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: the workspace is missing, too small (%zu < %zu) or not 256-byte aligned", workspace_bytes,
                     chunk_workspace(*o, tokens));
     if ((reinterpret_cast<uintptr_t>(d_qkv) | reinterpret_cast<uintptr_t>(d_key_pages) | reinterpret_cast<uintptr_t>(d_value_pages) |
-         reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_rope_cos) | reinterpret_cast<uintptr_t>(d_rope_sin)) & 15)
-        return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: rows, cache pages, rope tables and output must be 16-byte aligned");
-    if ((reinterpret_cast<uintptr_t>(d_q_norm_weight) | reinterpret_cast<uintptr_t>(d_k_norm_weight)) & 3)
-        return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: the norm weights must be 4-byte aligned");
+         reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_rope_cos) | reinterpret_cast<uintptr_t>(d_rope_sin) |
+         reinterpret_cast<uintptr_t>(d_q_norm_weight) | reinterpret_cast<uintptr_t>(d_k_norm_weight)) & 15)
+        return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: rows, cache pages, norm weights, rope tables and output must be 16-byte aligned");
     if ((long long)physical_pages * o->page_size > 0x7fff0000ll || (long long)tokens * o->q_heads > 0x7fff0000ll)
         return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: more than 2^31 cache slots or query rows");
     Chunk p;
@@ -157,7 +178,18 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     p.width = o->max_logical_pages, p.physical_pages = physical_pages, p.max_context = o->max_context;
     p.eps = o->norm_eps;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    GB_CUDA(chunk_launch(attn_chunk_rows_kernel, dim3(unsigned(tokens)), s, (flags & 1u) != 0, p));
+    const long long warps = (long long)tokens * ((o->q_heads + 2 * o->kv_heads + 3) / 4), ctas = (warps * 32 + kRowThreads - 1) / kRowThreads;
+    if (ctas > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: too many rows");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(ctas));
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = (flags & 1u) ? 1 : 0;
+    GB_CUDA(cudaLaunchKernelEx(&cfg, attn_chunk_rows_kernel, p, int(ctas <= 2 * kSmCount)));
     return chunk_attention_launch(p, s);
 }
 

@@ -335,7 +335,7 @@ int garnet_b200_attention_decode(const garnet_b200_attention_options* options, c
  *   - Slots whose page is not one of the `physical_pages` of the cache are not written and not seen; a row that sees none is zeros.
  *   - What the cache holds behind a sequence's last slot does not matter (NaN and infinities included).
  *   - Pages that hold the slots of new rows belong to one sequence each; full pages before them may be shared.
- *   - q_heads / kv_heads at most 128.
+ *   - q_heads / kv_heads at most 128.  Rows, cache pages, norm weights, rope tables and output start on 16-byte boundaries.
  * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned) needs no clearing and holds nothing
  * between calls; calls that overlap on the GPU need one each.  flags bit 0: programmatic dependent launch.  No allocation, no
  * synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step
