@@ -48,14 +48,15 @@ struct ChShape {
     // warps are allocated four at a time: 14, as well as twice 8, leave a thread 128 registers
     static constexpr int softmax_warps = 4 * kTiles, mma_warp = softmax_warps, scout_warp = mma_warp + kTiles, load_warp = scout_warp + kTiles, loaders = 2;
     static constexpr int threads = (load_warp + loaders) * 32;
-    static constexpr int ahead = kUnits > 2 ? 3 : 1;                      // units under way when the next is asked for
+    static constexpr int ahead = kUnits > 2 ? kUnits - 2 : 1;                      // units under way when the next is asked for
     static constexpr int q_half = kChRows * 128, q_tile = 2 * q_half;    // 64 dims of a tile of queries; all of them
     static constexpr int half = kKeys * 128, slot = 2 * half, unit = 2 * slot;   // the same of a step's keys (or values); keys and values
     static constexpr int q = 0, ring = kTiles * q_tile, exists = ring + kUnits * unit, bars = exists + kChExists * kChRounds * 4;
     static constexpr int total = bars + 512 + 1024;                      // barriers, and slack for 1024-byte alignment
-    // partial results of a split call, over the queries and the ring: rows of 128 floats, 16 bytes apart in the banks; maxima, sums
-    static constexpr int part_row = (kChDim + 4) * 4, stats = kTiles * kChRows * part_row;
-    static_assert(stats + kTiles * kChRows * 8 <= exists, "the partial results fit where the queries and the ring were");
+    // the parts of the rows that this CTA of a split call finishes, over the queries and the ring: [row][CTA] rows of 128 floats, 16 bytes
+    // apart in the banks; maxima and sums
+    static constexpr int part_row = (kChDim + 4) * 4, parts = kTiles * kChRows + 8, stats = parts * part_row;
+    static_assert(stats + parts * 8 <= exists, "the parts fit where the queries and the ring were");
     static_assert(total <= 227 * 1024, "shared memory budget");
     // tensor memory of a tile: two sets of scores (P replaces them), O
     static constexpr uint32_t col_o = 2 * kKeys, tile_cols = col_o + kChDim, cols = kTiles * tile_cols;
@@ -111,7 +112,7 @@ __device__ __forceinline__ ChBlock chunk_block(const Chunk& p, int y, int rows, 
 }
 
 template <int kTiles, int kUnits>
-__global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 ? 2 : 1)
+__global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 ? 2 : 1)
     attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
 {
     using S = ChShape<kTiles, kUnits>;
@@ -339,10 +340,17 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
         // steps in which the tiles take turns with their exponentials: left alone they fall into step, first both on the exponential
         // unit, then neither
         const int turns = kTiles == 2 ? min(steps[0], steps[kTiles - 1]) : 0;
+        const bool any = __any_sync(0xffffffffu, end > 0);
         for (int j = 0; j < my_steps; ++j) {
             const int kb = (step0 + j) * kKeys;
             const uint32_t ts = tm + (j & 1) * kKeys;
             scores_of(j);
+            if (!any) {   // none of the warp's rows sees a key: their weights may be what they are
+                if (j < turns && (q == 1 || j > 0)) bar_sync(kBarTurn + q, 256);
+                if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
+                bar_arrive(kBarP + q * 2 + (j & 1), 160);
+                continue;
+            }
             tc_fence_after();
             uint32_t s[kChRounds][32];
 #pragma unroll
@@ -457,8 +465,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
                 chunk_row(p, blk.b, __shfl_sync(0xffffffffu, blk.row0 + t, from), __shfl_sync(0xffffffffu, head, from), __shfl_sync(0xffffffffu, end, from) - 1, lane);
             }
         } else {
-            __syncthreads();   // all of the CTA's copies and MMAs are done: their operands may be written over
-            float* row = reinterpret_cast<float*>(smem + (q * kChRows + r) * S::part_row);
+            // Row i is finished by CTA i % splits of the cluster: its part goes there, as row i / splits.
+            cg::cluster_group cluster = cg::this_cluster();
+            cluster.sync();   // every CTA's copies and MMAs are done: their operands may be written over
+            const int i = q * kChRows + r, at = i / splits * splits + split;
+            uint8_t* there = reinterpret_cast<uint8_t*>(cluster.map_shared_rank(smem, i % splits));
 #pragma unroll 1
             for (int c = 0; c < kChDim / 32; ++c) {
                 uint32_t o[32];
@@ -468,53 +479,64 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kTiles == 1 
                 }
                 if (mine) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(row + 32 * c + 4 * i) = my_steps ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0, 0, 0, 0);
+                    for (int k = 0; k < 8; ++k)
+                        *reinterpret_cast<uint4*>(there + at * S::part_row + (32 * c + 4 * k) * 4) = my_steps ? make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]) : make_uint4(0, 0, 0, 0);
                 }
             }
-            *reinterpret_cast<float2*>(smem + S::stats + (q * kChRows + r) * 8) = make_float2(my_steps ? ref : -INFINITY, my_steps ? sum : 0.f);
+            if (mine) *reinterpret_cast<float2*>(there + S::stats + at * 8) = make_float2(my_steps ? ref : -INFINITY, my_steps ? sum : 0.f);
         }
     }
     if (splits > 1) {
-        // ---- the CTAs' partial results; the rows go round the cluster's warps
-        if (warp >= S::softmax_warps) __syncthreads();   // with the softmax warps above
         cg::cluster_group cluster = cg::this_cluster();
+        if (warp >= S::softmax_warps) cluster.sync();   // with the softmax warps above
         cluster.sync();
+        // ---- this CTA's rows from the parts of all: four rows to a warp, eight lanes each
         constexpr int kWarps = S::threads / 32;
-        for (int i = split * kWarps + warp; i < kTiles * kChRows; i += splits * kWarps) {
+        const int most_rows = (kTiles * kChRows - split + splits - 1) / splits, l = lane & 7;
+        for (int base = warp * 4; base < most_rows; base += kWarps * 4) {
+            const int local = min(base + (lane >> 3), most_rows - 1), i = local * splits + split;
             const int q = i / kChRows, r = i % kChRows, in_tile = r / group, t = blk.first + q * tile_tokens + in_tile, head = kv * group + r % group;
-            if (in_tile >= tile_tokens || t >= blk.len) continue;
-            const int end = blk.pos0 < 0 || blk.pos0 > p.max_context - 1 - t ? 0 : blk.pos0 + t + 1;
-            float2 st[kChMaxSplits];
-            float4 part[kChMaxSplits];
+            const bool mine = base + (lane >> 3) < most_rows && in_tile < tile_tokens && t < blk.len;
+            const int end = !mine || blk.pos0 < 0 || blk.pos0 > p.max_context - 1 - t ? 0 : blk.pos0 + t + 1;
+            const float2 st = l < splits ? *reinterpret_cast<const float2*>(smem + S::stats + (local * splits + l) * 8) : make_float2(-INFINITY, 0.f);
+            float top = st.x;
 #pragma unroll
-            for (int c = 0; c < kChMaxSplits; ++c) {
-                const int from = c < splits ? c : 0;
-                st[c] = *reinterpret_cast<const float2*>(cluster.map_shared_rank(smem + S::stats + i * 8, from));
-                part[c] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(smem + i * S::part_row + lane * 16, from));
-                if (c >= splits) st[c] = make_float2(-INFINITY, 0.f);
+            for (int d = 1; d < kChMaxSplits; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float f = st.y == 0.f ? 0.f : ex2(st.x - top);   // 0: nothing visible there
+            float total = f * st.y;
+#pragma unroll
+            for (int d = 1; d < kChMaxSplits; d <<= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            const float factor = total == 0.f || end == 0 ? 0.f : f / total;
+            float4 o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int c = 0; c < splits; ++c) {
+                const float w = __shfl_sync(0xffffffffu, factor, (lane & 24) + c);
+                const float4* from = reinterpret_cast<const float4*>(smem + (local * splits + c) * S::part_row) + l;
+                if (w == 0.f) continue;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = from[8 * k];
+                    o[k].x += w * v.x, o[k].y += w * v.y, o[k].z += w * v.z, o[k].w += w * v.w;
+                }
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < kChMaxSplits; ++c) top = fmaxf(top, st[c].x);
-            float total = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int c = 0; c < kChMaxSplits; ++c) {
-                if (st[c].y == 0.f) continue;   // nothing visible there
-                const float f = ex2(st[c].x - top);
-                total += f * st[c].y;
-                o.x += f * part[c].x, o.y += f * part[c].y, o.z += f * part[c].z, o.w += f * part[c].w;
-            }
-            const float inv = end == 0 || total == 0.f ? 0.f : 1.f / total;
-            o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+            bool bad = false;
             const int row = blk.row0 + t;
-            *reinterpret_cast<uint2*>(p.out + (size_t(row) * p.q_heads + head) * kChDim + lane * 4) = make_uint2(bf16x2_of(o.x, o.y), bf16x2_of(o.z, o.w));
-            const bool bad = isnan(o.x) || isnan(o.y) || isnan(o.z) || isnan(o.w);
+            if (mine) {
+                uint2* out = reinterpret_cast<uint2*>(p.out + (size_t(row) * p.q_heads + head) * kChDim) + l;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    bad = bad || isnan(o[k].x) || isnan(o[k].y) || isnan(o[k].z) || isnan(o[k].w);
+                    out[8 * k] = make_uint2(bf16x2_of(o[k].x, o[k].y), bf16x2_of(o[k].z, o[k].w));
+                }
+            }
             __syncwarp();
-            if (__any_sync(0xffffffffu, bad) && !*abort_flag) chunk_row(p, blk.b, row, head, end - 1, lane);
+            const uint32_t redo = __ballot_sync(0xffffffffu, bad);
+            if (redo && !*abort_flag)
+                for (int g = 0; g < 4; ++g)
+                    if ((redo >> (8 * g)) & 0xffu)
+                        chunk_row(p, blk.b, __shfl_sync(0xffffffffu, row, 8 * g), __shfl_sync(0xffffffffu, head, 8 * g), __shfl_sync(0xffffffffu, end, 8 * g) - 1, lane);
         }
-        cluster.sync();   // peers may still read this CTA's results
     }
     tc_fence_before();
     __syncthreads();
@@ -557,7 +579,8 @@ int launch(const Chunk& p, int splits, cudaStream_t stream)
 int chunk_attention_launch(const Chunk& p, cudaStream_t stream)
 {
     const ChunkPlan plan = chunk_plan(p.batch, p.kv_heads, p.tokens, kChRows / (p.q_heads / p.kv_heads), p.max_context);
-    return plan.tiles == 2 ? launch<2, 5>(p, plan.splits, stream) : launch<1, 2>(p, plan.splits, stream);
+    if (plan.tiles == 2) return launch<2, 5>(p, plan.splits, stream);
+    return plan.units == 2 ? launch<1, 2>(p, plan.splits, stream) : launch<1, 6>(p, plan.splits, stream);
 }
 
 }  // namespace gb200
