@@ -41,7 +41,7 @@ __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("ba
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int kKeys = 64;         // keys of a step (UMMA N of Q K^T, K of P V)
 constexpr int kChRounds = kKeys / 32;   // P is handed over, and rows are copied, 32 keys at a time
-constexpr int kChExists = 8;      // steps whose key bits are kept: more than the ring holds
+constexpr int kChExists = 16;     // steps whose key bits are kept
 
 template <int kTiles, int kUnits>
 struct ChShape {
@@ -58,6 +58,8 @@ struct ChShape {
     static constexpr int part_row = (kChDim + 4) * 4, parts = kTiles * kChRows + 8, stats = parts * part_row;
     static_assert(stats + parts * 8 <= exists, "the parts fit where the queries and the ring were");
     static_assert(total <= 227 * 1024, "shared memory budget");
+    // the key bits of step u are written when unit u - kUnits - 1 is done, and with it the softmax of two steps before that
+    static_assert(kUnits + 3 <= kChExists, "key bits");
     // tensor memory of a tile: two sets of scores (P replaces them), O
     static constexpr uint32_t col_o = 2 * kKeys, tile_cols = col_o + kChDim, cols = kTiles * tile_cols;
     static_assert(kTiles * tile_cols <= 512, "tensor memory");
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     using S = ChShape<kTiles, kUnits>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint32_t* exists = reinterpret_cast<uint32_t*>(smem + S::exists);       // [4 steps][kChRounds]: bits of the keys that have a page
+    uint32_t* exists = reinterpret_cast<uint32_t*>(smem + S::exists);       // [steps][kChRounds]: bits of the keys that have a page
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::bars);           // [units]
     uint64_t* empty = full + kUnits;                                        // [units]
     uint64_t* q_full = empty + kUnits;
@@ -242,7 +244,6 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                     const bool there = page[u] >= 0 && page[u] < p.physical_pages;
                     row[u] = there ? page[u] * p.page_size + within[u] : -1;
                     const uint32_t bits = __ballot_sync(0xffffffffu, there);
-                    // which keys there are: the softmax of eight steps before has long been done when the ring takes this one
                     if (lane == 0 && u * S::loaders + lw < kChRounds) exists[(sent % kChExists) * kChRounds + u * S::loaders + lw] = bits;
                 }
                 look_up(sent + 1);   // asked for a step ahead
