@@ -26,8 +26,8 @@ class PagePool:
         if not keys or len(keys) != len(values):
             raise ValueError("PagePool needs as many layers of key pages as of value pages")
         shape = keys[0].shape
-        if len(shape) < 3:
-            raise ValueError("the pages of a layer must be [pages, page_size, ...]")
+        if len(shape) < 3 or 0 in shape:
+            raise ValueError("the pages of a layer must be [pages, page_size, ...], none of them empty")
         for i, t in enumerate(keys + values):
             on_device(t, f"the pages of layer {i % len(keys)}", keys[0].dtype, tuple(shape))
         self._keep = keys, values

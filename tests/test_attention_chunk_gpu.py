@@ -179,6 +179,19 @@ def test_batches_that_fill_the_gpu(q_heads, kv_heads, lens, starts, page_size):
     Case(lens, starts, q_heads, kv_heads, page_size=page_size, pad=2, seed=q_heads).check()
 
 
+@pytest.mark.parametrize("batch,q_heads,kv_heads,tokens,start", [
+    (1, 2, 1, 1, 0), (16, 8, 8, 1, 1500), (6, 8, 8, 1, 500), (1, 2, 1, 1, 500),
+    (16, 8, 8, 1, 300), (3, 8, 8, 300, 500), (16, 6, 2, 1, 3000), (1, 2, 1, 1, 4500),
+    (16, 8, 8, 130, 500), (6, 8, 8, 130, 1500), (3, 8, 8, 130, 3000), (6, 6, 2, 64, 4500)])
+def test_every_kind_of_cta_and_share_of_keys(batch, q_heads, kv_heads, tokens, start):
+    """One tile with a short or a long ring, two tiles; keys in 1, 2, 4 or 8 shares; contexts with pages missing here and there, the first
+    third of one missing altogether, so that shares of it hold nothing."""
+    c = Case([tokens] * batch, [start] * batch, q_heads, kv_heads, seed=batch + tokens)
+    c.table[:, 3::7] = -1
+    c.table[0, :start // 48] = -1
+    c.check()
+
+
 def test_sharp_scores():
     """Scores of some hundreds: all weight on single positions, maxima that grow from tile to tile, rows whose largest score comes last."""
     c = Case([140], [400], 2, 1, seed=5)

@@ -268,7 +268,7 @@ def test_refusals():
                 lambda: pool.fork(ints([0]), ints([[1]])), lambda: pool.free(torch.zeros(1, dtype=torch.int32)), lambda: pool.free(ints([0] * 5)),
                 lambda: pool.copy_pages(ints([0, 1]), ints([1])), lambda: cache.PagePool(keys, values + values, 4, 4), lambda: cache.PagePool([], [], 4, 4),
                 lambda: cache.PagePool([keys[0].cpu()], values, 4, 4), lambda: cache.PagePool([keys[0].transpose(0, 1)], values, 4, 4),
-                lambda: cache.PagePool([keys[0][:4]], values, 4, 4)):
+                lambda: cache.PagePool([keys[0][:4]], values, 4, 4), lambda: cache.PagePool([keys[0][:0]], [values[0][:0]], 4, 4)):
         with pytest.raises(ValueError):
             bad()
     with pytest.raises(garnet_b200.GarnetB200Error):       # 8 bytes per position

@@ -48,3 +48,10 @@ def test_plan_follows_the_work(plan):
     assert long_one == (1, 6, 8)       # few rows, many keys: a deep ring
     assert piece == (2, 5, 4)
     assert prompt == (2, 5, 1)         # enough tiles for every SM: keys are not shared out
+
+
+def test_every_kind_is_taken_somewhere(plan):
+    kinds = {(1, 2, n) for n in (1, 2, 4, 8)} | {(1, 6, n) for n in (1, 2, 4, 8)} | {(2, 5, n) for n in (1, 2, 4, 8)}
+    cases = [(b, kv, b * t, tile, -(-(s + t) // 16) * 16 + 16) for b in (1, 3, 6, 16) for kv, tile in ((1, 64), (8, 64), (8, 128), (2, 42))
+             for t in (1, 64, 130, 300) for s in (0, 500, 1500, 3000, 4500)]
+    assert set(plan(cases)) == kinds
