@@ -8,31 +8,33 @@
 #include <cstdint>
 
 #include "attn_chunk.cuh"
+#include "tc_common.cuh"
 
 namespace gb200 {
 
 namespace {
 
-// a cos + b sin with one rounding's error: the second product's own is added back.
-__device__ __forceinline__ float turned(float a, float cosine, float b, float sine)
+// a cos + b sin of two values at once with one rounding's error: what the second product is short of is added back.
+__device__ __forceinline__ uint64_t turned(uint64_t a, uint64_t cosine, uint64_t b, uint64_t sine, uint64_t minus_sine)
 {
-    const float p = __fmul_rn(b, sine);
-    return __fadd_rn(__fmaf_rn(a, cosine, p), __fmaf_rn(b, sine, -p));
+    const uint64_t p = mul2(b, sine);
+    return fma2(fma2(b, minus_sine, p), f32x2(-1.f, -1.f), fma2(a, cosine, p));
 }
-__device__ __forceinline__ void unpack(const uint4& v, float* x)
+// two bf16 numbers as two fp32 numbers; and rounded back
+__device__ __forceinline__ uint64_t wide(uint32_t w) { return f32x2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t narrow(uint64_t v)
 {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    float lo, hi;
+    f32x2_split(v, lo, hi);
+    return bf16x2_of(lo, hi);
 }
-__device__ __forceinline__ uint4 pack(const float* x) { return make_uint4(bf16x2_of(x[0], x[1]), bf16x2_of(x[2], x[3]), bf16x2_of(x[4], x[5]), bf16x2_of(x[6], x[7])); }
 
 // A warp takes four heads of a row, eight lanes each: dims 8 l .. 8 l + 7 and the eight 64 further on, which RoPE turns together.
 // Rounded to bf16 after the norm and after the rotation, as a bf16 network does; the fp32 steps in between carry what the sum of
 // squares, the products and the root are short of: some 1 of 10^6 results is the other bf16 neighbour of the float64 result (10 to
 // 20 of 10^6 by plain fp32 steps).
-// Bound: HBM, the rows in and q, k and v out.  8192 rows of 16 / 8 heads: 60 us with a CTA per row, a warp per head and the sums in
-// double.
+// Bound: HBM in principle, the rows in and q, k and v out; in practice its instructions, some 250 for four heads with two values to an
+// instruction.
 constexpr int kRowThreads = 256;
 __global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const Chunk p, const int early)
 {
@@ -70,14 +72,23 @@ __global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const C
         if (at >= 0) to = reinterpret_cast<uint4*>((turns ? p.keys : p.values) + at);
     }
     if (__any_sync(0xffffffffu, turns)) {
-        float x[16], w[16];
-        unpack(lo, x), unpack(hi, x + 8), unpack(wlo, w), unpack(whi, w + 8);
-        float sum = 0.f, rest = 0.f;   // the sum of squares and what it is short of
+        // packed: dims 8 l + 2 i, 8 l + 2 i + 1, and from i = 4 on those 64 further on
+        const uint32_t xs[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, ws[8] = {wlo.x, wlo.y, wlo.z, wlo.w, whi.x, whi.y, whi.z, whi.w};
+        const uint64_t minus1 = f32x2(-1.f, -1.f);
+        uint64_t sum2 = 0, rest2 = 0;   // the sum of squares and what it is short of
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float next = __fmaf_rn(x[i], x[i], sum);
-            rest = __fadd_rn(rest, __fmaf_rn(x[i], x[i], -__fsub_rn(next, sum)));
-            sum = next;
+        for (int i = 0; i < 8; ++i) {
+            const uint64_t x = wide(xs[i]), next = fma2(x, x, sum2);
+            rest2 = add2(rest2, fma2(x, x, fma2(next, minus1, sum2)));
+            sum2 = next;
+        }
+        float sum, rest;
+        {
+            float s0, s1, r0, r1;
+            f32x2_split(sum2, s0, s1), f32x2_split(rest2, r0, r1);
+            const float a = fmaxf(s0, s1), c = fminf(s0, s1);
+            sum = __fadd_rn(a, c);
+            rest = r0 + r1 + __fsub_rn(c, __fsub_rn(sum, a));
         }
 #pragma unroll
         for (int off = 4; off; off >>= 1) {
@@ -91,20 +102,24 @@ __global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const C
         const float r = 1.f / sqrtf(mean), square = __fmul_rn(mean, r);
         // what r is short of 1 / sqrt(mean)
         const float c = 0.5f * r * (__fmaf_rn(-square, r, 1.f) - __fmaf_rn(mean, r, -square) * r - short_of * r * r);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float v = __fmul_rn(x[i], w[i]);   // exact: two bf16 numbers
-            x[i] = bf16_round_f(__fmaf_rn(v, r, __fmul_rn(v, c)));
-        }
         if (turns) {
-            float y[16];
+            const uint64_t r2 = f32x2(r, r), c2 = f32x2(c, c);
+            uint64_t n[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float cosine = reinterpret_cast<const float*>(cs)[i], sine = reinterpret_cast<const float*>(sn)[i];
-                y[i] = turned(x[i], cosine, -x[i + 8], sine);
-                y[i + 8] = turned(x[i + 8], cosine, x[i], sine);
+                const uint64_t v = mul2(wide(xs[i]), wide(ws[i]));   // exact: products of two bf16 numbers
+                n[i] = wide(narrow(fma2(v, r2, mul2(v, c2))));
             }
-            lo = pack(y), hi = pack(y + 8);
+            uint32_t y[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* cosine = reinterpret_cast<const float*>(cs) + 2 * i;
+                const float* sine = reinterpret_cast<const float*>(sn) + 2 * i;
+                const uint64_t c2 = f32x2(cosine[0], cosine[1]), s2 = f32x2(sine[0], sine[1]), m2 = f32x2(-sine[0], -sine[1]);
+                y[i] = narrow(turned(n[i], c2, n[i + 4], m2, s2));
+                y[i + 4] = narrow(turned(n[i + 4], c2, n[i], s2, m2));
+            }
+            lo = make_uint4(y[0], y[1], y[2], y[3]), hi = make_uint4(y[4], y[5], y[6], y[7]);
         }
     }
     if (to) to[l] = lo, to[8 + l] = hi;

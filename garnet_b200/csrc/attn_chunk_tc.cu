@@ -1,20 +1,28 @@
 // Chunk attention over the paged cache on the tensor cores: S = Q K^T and O += P V as tcgen05 MMAs, the softmax in fp32.
 //
 // A CTA owns one kv head and one or two tiles of 128 query rows; a tile's rows are (token, q head of the group), so that the K and V
-// rows it stages serve all the q heads of the group.  Per step of 128 (or 64) keys:
-//   loader warps    look up the page of every key and copy its K and V rows by cp.async into a ring of slots: two halves of 64 dims,
-//                   128-byte rows, swizzled - the K-major operand of Q K^T and the MN-major operand of P V.  Rows that do not exist,
-//                   and those behind the last key that a row of the CTA sees, are filled with zeros (what the cache holds there
-//                   could be NaN).  TMA boxes of a page took the loader 120 clocks each to ask for (16 rows x 128 bytes; 4000 clocks
-//                   per step of 128 keys, more than all the rest);
-//   MMA warps       one thread per tile: P V of 32 keys when their P is there, after the last ones Q K^T of the next step: the tensor
-//                   pipe works on one tile while the other tile's softmax runs;
+// rows it stages serve all the q heads of the group.  Per step of 64 keys:
+//   loader warps    look up the page of every key and copy its K and V rows by cp.async into a ring of units (the keys of step u, the
+//                   values of step u - 2): halves of 64 dims, 128-byte rows, swizzled - the K-major operand of Q K^T and the MN-major
+//                   operand of P V.  Rows that do not exist, and those behind the last key that a row of the CTA sees, are filled
+//                   with zeros (what the cache holds there could be NaN).  TMA boxes of a page took the loader 120 clocks each to ask
+//                   for (16 rows x 128 bytes; 4000 clocks per 128 keys, more than all the rest);
+//   MMA warps       one thread per tile: P V of step u - 2, then the scores of step u into the set that its P leaves;
+//   scout warps     one per tile: wait for the MMAs' barrier in shared memory and pass it on to a named one;
 //   softmax warps   one thread per query row: scores into registers, running maximum, p = 2^(s c - m c), the row's sum in fp32, P as
 //                   bf16 over the scores in tensor memory; O stays in tensor memory and is rescaled only when a row's maximum has
-//                   grown by more than 2^8 since the last time (the final division makes that exact; the conditional rescaling of
-//                   FlashAttention-4).  The fp32 work runs two values per instruction.
-// Few rows after a long context: a cluster of up to 8 CTAs shares the keys, and their partial results meet in distributed shared
-// memory; every CTA finishes some of the rows.
+//                   grown by more than 2^8 since the last time (the final division makes that exact).  The fp32 work runs two
+//                   values per instruction.  Two tiles take turns with their exponentials.
+// Few rows after a long context: a cluster of up to 8 CTAs shares the keys; every CTA sends its part of row i to CTA i % splits by
+// stores to distributed shared memory, which joins and writes it (launch_plan.h says when).
+//
+// Bound: a step of two tiles costs 1024 clocks of the exponential unit (16 per clock) and 1330 of the tensor pipe (N = 64 takes 50
+// clocks per MMA instead of 33: both operands come from shared memory); it takes 1800 (0.95 us), the chain scores -> maximum -> exponentials
+// (780 clocks a tile, one after the other) -> P V.  B200, 16 / 8 heads: a prompt of 8192 tokens 287 us (0.57 of the measured bf16 peak
+// over the visible pairs, the rows kernel's 25 us included), 512 tokens at 30000 132 us, a prompt of 2048 46 us, 24 x 5 tokens at up to
+// 3500 65 us (0.46 of the measured bandwidth), 4 tokens at 1000 10.8 us.  Steps of 128 keys with one set of scores (MMAs of N = 128,
+// P handed over in pieces of 32 keys, with 128 or 192 registers to a softmax thread) took 293 to 300 us for 8192 tokens; part of the
+// exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
 // Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  P is rounded to bf16 where it meets V, 2^-8 of each
 // weight at most: the errors of the weights are independent of one another, so that a result is off by about what its own rounding
 // to bf16 takes (P in two pieces would cost half as many MMAs again).  A row that comes out NaN (infinities in places that it does not
