@@ -28,7 +28,7 @@ from typing import NamedTuple, Optional
 import numpy as np
 import torch
 
-from ._lib import BF16, FP16, FP32, check, lib, on_device, stream_ptr
+from ._lib import BF16, FP16, FP32, all_on_device, check, lib, on_device, stream_ptr
 from .linear import GlueList, W4A16Linear
 
 
@@ -105,21 +105,17 @@ class ChunkAttention:
                       max_logical_pages, cfg.q_heads * cfg.head_dim)
 
     def run(self, qkv, q_norm_w, k_norm_w, cos, sin, key_pages, value_pages, page_tables, positions, row_starts, out, pdl: bool = False):
-        bf, i32, d = torch.bfloat16, torch.int32, self._dims
-        rows, batch, pages = qkv.shape[0], positions.numel(), key_pages.shape[0]
-        on_device(qkv, "qkv", bf, (rows, d[0]))
-        on_device(q_norm_w, "q_norm_w", bf, d[1])
-        on_device(k_norm_w, "k_norm_w", bf, d[1])
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            on_device(t, name, torch.float32, (t.shape[0], d[2]))
-            if t.shape[0] < d[3]:
-                raise ValueError(f"{name} has fewer than {d[3]} rows")
-        on_device(key_pages, "key_pages", bf, (pages, *d[4]))
-        on_device(value_pages, "value_pages", bf, (pages, *d[4]))
-        on_device(page_tables, "page_tables", i32, (batch, d[5]))
-        on_device(positions, "positions", i32, (batch,))
-        on_device(row_starts, "row_starts", i32, (batch + 1,))
-        on_device(out, "out", bf, (rows, d[6]))
+        bf, f32, i32, d = torch.bfloat16, torch.float32, torch.int32, self._dims
+        rows, batch, pages, angles = qkv.shape[0], positions.numel(), key_pages.shape[0], cos.shape[0]
+        tensors = ((qkv, bf, (rows, d[0])), (q_norm_w, bf, d[1]), (k_norm_w, bf, d[1]), (cos, f32, (angles, d[2])), (sin, f32, (sin.shape[0], d[2])),
+                   (key_pages, bf, (pages, *d[4])), (value_pages, bf, (pages, *d[4])), (page_tables, i32, (batch, d[5])),
+                   (positions, i32, (batch,)), (row_starts, i32, (batch + 1,)), (out, bf, (rows, d[6])))
+        if not all_on_device(tensors, torch.cuda.current_device()):
+            names = ("qkv", "q_norm_w", "k_norm_w", "cos", "sin", "key_pages", "value_pages", "page_tables", "positions", "row_starts", "out")
+            for name, (t, dtype, shape) in zip(names, tensors):
+                on_device(t, name, dtype, shape)
+        if angles < d[3] or sin.shape[0] < d[3]:
+            raise ValueError(f"cos and sin must have {d[3]} rows or more")
         if self.ws.get_device() != qkv.get_device():
             raise ValueError("the workspace is on another device than the rows")
         if batch and rows:
@@ -162,23 +158,25 @@ def log_probs(logits, targets=None, top_k: int = 0, temperature: float = 1.0, pd
     stride, step = logits.stride()
     if rows <= 1:
         stride = vocab
-    device = logits.device
-    if device.type != "cuda" or device.index != torch.cuda.current_device() or (vocab > 1 and step != 1) or stride < vocab:
+    index = logits.get_device()
+    if index < 0 or index != torch.cuda.current_device() or (vocab > 1 and step != 1) or stride < vocab:
         raise ValueError("log_probs needs rows of neighbouring values on the current CUDA device")
-    f32, i32, k = torch.float32, torch.int32, max(0, top_k)
+    k = max(0, top_k)
+    # the results of a small call take longer to allocate than to compute: like one another they take less
+    entropy = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    top = entropy.new_empty(rows, k)
+    ids = torch.empty_like(top, dtype=torch.int32)
     log_prob = rank = None
+    given = (None, None, None)
     if targets is not None:
-        on_device(targets, "targets", i32, (rows,))
-        log_prob, rank = torch.empty(rows, dtype=f32, device=device), torch.empty(rows, dtype=i32, device=device)
-    r = LogProbs(log_prob, rank, torch.empty(rows, dtype=f32, device=device), torch.empty(rows, k, dtype=f32, device=device),
-                 torch.empty(rows, k, dtype=i32, device=device))
+        on_device(targets, "targets", torch.int32, (rows,))
+        log_prob, rank = torch.empty_like(entropy), torch.empty_like(targets)
+        given = targets.data_ptr(), log_prob.data_ptr(), rank.data_ptr()
     if rows:
-        given = targets is not None
-        check(lib().garnet_b200_log_probs(logits.data_ptr(), kind, stride, targets.data_ptr() if given else None, rows, vocab, top_k, temperature,
-                                          log_prob.data_ptr() if given else None, rank.data_ptr() if given else None, r.entropy.data_ptr(),
-                                          r.top_log_probs.data_ptr() if k else None, r.top_ids.data_ptr() if k else None, 1 if pdl else 0,
+        check(lib().garnet_b200_log_probs(logits.data_ptr(), kind, stride, given[0], rows, vocab, top_k, temperature, given[1], given[2],
+                                          entropy.data_ptr(), top.data_ptr() if k else None, ids.data_ptr() if k else None, 1 if pdl else 0,
                                           stream_ptr()))
-    return r
+    return LogProbs(log_prob, rank, entropy, top, ids)
 
 
 class DecodeStep:
