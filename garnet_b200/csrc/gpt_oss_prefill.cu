@@ -13,8 +13,8 @@
 //   2 x 4 softmax     one thread per query row: 64 scores into registers, running maximum (the sink is its first value),
 //   warps             p = 2^(s c - m c), the row's sum in fp32, P over the scores in tensor memory; the P V of the step before
 //                     is added to O, which stays in registers and is rescaled only when a row's maximum has grown by more than
-//                     2^8 since the last time (the final division makes that exact; the conditional rescaling of
-//                     FlashAttention-4).  The fp32 work runs two values per instruction (f32x2).
+//                     2^8 since the last time (the final division makes that exact).  The fp32 work runs two values per
+//                     instruction (f32x2).
 // Numerics: the queries are bf16-valued fp32, so Q K^T has exact products; the queries of a CTA that holds others enter as three
 // bf16 numbers each.  P is fp32 and enters the MMA as three bf16 numbers, which hold eight of its 24 bits each.  The tensor core
 // truncates what it accumulates, so a sum that stays in it loses about half a unit of its last place per MMA: each step starts a

@@ -15,7 +15,9 @@
 // Everything is added in an order that depends on sizes only.  A row whose maximum lies beyond +-2^100 (a mask of the type's lowest
 // value over all of it) or, in y, beyond +-2^20 (a temperature next to zero) is summed again, value by value, against its maximum.
 //
-// Bound: HBM in principle (every logit once); for 16-bit logits the exponentials, 16 per clock and SM, take longer.
+// Bound: HBM in principle (every logit once).  For 16-bit logits the exponentials, 16 per clock and SM, take nearly as long (69 of 95 us for
+// 2048 rows of 151936): that call takes 125 us, 0.76 of the measured bandwidth, the exponential unit busy 64 % of it.  One row of 151936 and
+// 64 rows of 32003 fp32 take 11.5 us each, the latency of launch, loads, two meetings of the cluster and the alternatives' order.
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
