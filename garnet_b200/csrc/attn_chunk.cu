@@ -36,13 +36,79 @@ __device__ __forceinline__ uint32_t narrow(uint64_t v)
 // Bound: HBM in principle, the rows in and q, k and v out; in practice its instructions, some 250 for four heads with two values to an
 // instruction.
 constexpr int kRowThreads = 256;
+
+// One CTA beside the rows': the attention's blocks of rows by the keys that they see, the most first, so that the last CTAs to start
+// are short ones (24 ragged sequences of 5 rows at up to 3500: 47 instead of 65 us, a ragged batch of 8 prompts 58 instead of 74 us with
+// the sequences in their own order).  A counting sort; blocks that see equally much (within 1 / 1023 of max_context) come in any order.
+constexpr int kOrderBuckets = 4 * kRowThreads;
+__device__ __forceinline__ void chunk_order(const Chunk& p)
+{
+    __shared__ int places[kOrderBuckets], sums[kRowThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = threadIdx.x; i < kOrderBuckets; i += kRowThreads) places[i] = 0;
+    __syncthreads();
+    const auto every_block = [&](auto&& take) {   // take(block, its bucket)
+        for (int b0 = 0; b0 < p.batch; b0 += kRowThreads) {
+            const int b = b0 + int(threadIdx.x);
+            int row0 = 0, len = 0, pos0 = 0;
+            if (b < p.batch) {
+                row0 = min(max(p.row_starts[b], 0), p.tokens);
+                len = min(max(p.row_starts[b + 1], row0), p.tokens) - row0;
+                pos0 = p.positions[b];
+            }
+            const int n = (len + p.block_rows - 1) / p.block_rows;
+            const auto one = [&](int b, int row0, int len, int pos0, int k) {
+                const int first = k * p.block_rows;
+                const long long end = pos0 < 0 || pos0 > p.max_context - 1 - first ? 0 : min((long long)p.max_context, (long long)pos0 + min(len, first + p.block_rows));
+                take(ChunkBlock{b, first, len, row0, pos0, {}}, kOrderBuckets - 1 - int(end * (kOrderBuckets - 1) / p.max_context));
+            };
+            if (n == 1) one(b, row0, len, pos0, 0);
+            for (uint32_t many = __ballot_sync(0xffffffffu, n > 1); many; many &= many - 1) {   // the warp together
+                const int from = __ffs(many) - 1, of = __shfl_sync(0xffffffffu, n, from), r0 = __shfl_sync(0xffffffffu, row0, from);
+                const int l = __shfl_sync(0xffffffffu, len, from), p0 = __shfl_sync(0xffffffffu, pos0, from);
+                for (int k = lane; k < of; k += 32) one(b0 + warp * 32 + from, r0, l, p0, k);
+            }
+        }
+    };
+    every_block([&](const ChunkBlock&, int bucket) { atomicAdd(&places[bucket], 1); });
+    __syncthreads();
+    // a bucket's first place: the blocks of those before it
+    int mine[4], total = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine[i] = total, total += places[4 * threadIdx.x + i];
+    int upto = total;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    int before = upto - total, all = 0;
+#pragma unroll
+    for (int w = 0; w < kRowThreads / 32; ++w) before += w < warp ? sums[w] : 0, all += sums[w];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) places[4 * threadIdx.x + i] = before + mine[i];
+    __syncthreads();
+    every_block([&](const ChunkBlock& block, int bucket) {
+        const int at = atomicAdd(&places[bucket], 1);
+        if (at < p.block_count) p.blocks[at] = block;   // lists that do not ascend may ask for more
+    });
+    for (int i = all + int(threadIdx.x); i < p.block_count; i += kRowThreads) p.blocks[i].b = -1;
+}
+
 __global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const Chunk p, const int early)
 {
     // few rows: the attention's CTAs come up beside these; many: they would only take their place
     if (early) pdl_launch_dependents();
     pdl_wait();
+    if (blockIdx.x == 0) {
+        chunk_order(p);
+        if (!early) pdl_launch_dependents();
+        return;
+    }
     const int lane = threadIdx.x & 31, l = lane & 7, heads = p.q_heads + 2 * p.kv_heads, quads = (heads + 3) / 4, group = p.q_heads / p.kv_heads;
-    const long long task = (long long)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+    const long long task = (long long)(blockIdx.x - 1) * (kRowThreads / 32) + (threadIdx.x >> 5);
     const int row = int(task / quads), h = int(task % quads) * 4 + (lane >> 3);
     if (row >= p.tokens) return;
     const bool has = h < heads, is_q = h < p.q_heads, turns = h < p.q_heads + p.kv_heads;
@@ -142,7 +208,9 @@ int validate_chunk(const garnet_b200_attention_options* o)
     return GARNET_B200_OK;
 }
 
-size_t chunk_workspace(const garnet_b200_attention_options& o, int tokens) { return size_t(tokens) * o.q_heads * kChDim * 2; }
+// queries, and a block's entry per row at most
+size_t chunk_queries(const garnet_b200_attention_options& o, int tokens) { return size_t(tokens) * o.q_heads * kChDim * 2; }
+size_t chunk_workspace(const garnet_b200_attention_options& o, int tokens) { return chunk_queries(o, tokens) + size_t(tokens) * sizeof(ChunkBlock); }
 
 }  // namespace
 
@@ -189,11 +257,17 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     p.tables = d_page_tables, p.positions = d_positions, p.row_starts = d_row_starts;
     p.out = static_cast<__nv_bfloat16*>(d_out);
     p.queries = static_cast<__nv_bfloat16*>(d_workspace);
+    p.blocks = reinterpret_cast<ChunkBlock*>(static_cast<char*>(d_workspace) + chunk_queries(*o, tokens));
     p.batch = batch, p.tokens = tokens, p.q_heads = o->q_heads, p.kv_heads = o->kv_heads, p.page_size = o->page_size;
     p.width = o->max_logical_pages, p.physical_pages = physical_pages, p.max_context = o->max_context;
     p.eps = o->norm_eps;
+    const int tile_tokens = kChTileRows / (o->q_heads / o->kv_heads);
+    const ChunkPlan plan = chunk_plan(batch, o->kv_heads, tokens, tile_tokens, o->max_context);
+    p.block_rows = tile_tokens * plan.tiles;
+    // blocks of a sequence's rows: ceil(rows / block) summed over the sequences, of whose lengths the host knows the sum's limit only
+    p.block_count = int(std::min<long long>(tokens, (long long)tokens / p.block_rows + batch));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const long long warps = (long long)tokens * ((o->q_heads + 2 * o->kv_heads + 3) / 4), ctas = (warps * 32 + kRowThreads - 1) / kRowThreads;
+    const long long warps = (long long)tokens * ((o->q_heads + 2 * o->kv_heads + 3) / 4), ctas = (warps * 32 + kRowThreads - 1) / kRowThreads + 1;
     if (ctas > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: too many rows");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(unsigned(ctas));
@@ -205,7 +279,7 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     cfg.attrs = attr;
     cfg.numAttrs = (flags & 1u) ? 1 : 0;
     GB_CUDA(cudaLaunchKernelEx(&cfg, attn_chunk_rows_kernel, p, int(ctas <= 2 * kSmCount)));
-    return chunk_attention_launch(p, s);
+    return chunk_attention_launch(p, plan, s);
 }
 
 }  // extern "C"

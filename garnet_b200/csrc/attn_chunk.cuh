@@ -5,6 +5,13 @@
 namespace gb200 {
 
 constexpr int kChDim = 128;
+constexpr int kChTileRows = 128;   // (token, q head of the group) rows of a tile of the attention
+
+// Rows that a CTA of the attention takes: tokens `first` .. of sequence b, which has `len` of them from row `row0` on, the first of
+// them at slot pos0; b is -1 where there is nothing to do.
+struct alignas(16) ChunkBlock {
+    int b, first, len, row0, pos0, unused[3];
+};
 
 struct Chunk {
     const __nv_bfloat16* qkv;        // [tokens, (q_heads + 2 kv_heads) * 128]
@@ -19,7 +26,9 @@ struct Chunk {
     const int* row_starts;           // [batch + 1]
     __nv_bfloat16* out;              // [tokens, q_heads * 128]
     __nv_bfloat16* queries;          // workspace: [kv head][token][q head of the group][128]
+    ChunkBlock* blocks;              // workspace: the attention's blocks of rows, those that see the most keys first
     int batch, tokens, q_heads, kv_heads, page_size, width, physical_pages, max_context;
+    int block_rows, block_count;     // tokens of a block; entries of `blocks`
     float eps;
 };
 
@@ -84,7 +93,8 @@ __device__ __forceinline__ void chunk_row(const Chunk& p, int b, int row, int he
 
 #endif
 
-// attn_chunk_tc.cu: the attention of rows whose queries lie in the workspace and whose keys and values lie in the cache.
-int chunk_attention_launch(const Chunk& p, cudaStream_t stream);
+struct ChunkPlan;
+// attn_chunk_tc.cu: the attention of rows whose queries and blocks lie in the workspace and whose keys and values lie in the cache.
+int chunk_attention_launch(const Chunk& p, const ChunkPlan& plan, cudaStream_t stream);
 
 }  // namespace gb200

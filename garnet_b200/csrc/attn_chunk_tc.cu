@@ -39,7 +39,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kChRows = 128;      // query rows of a tile (UMMA M, one softmax thread each)
+constexpr int kChRows = kChTileRows;   // query rows of a tile (UMMA M, one softmax thread each)
 constexpr int kChMaxSplits = 8;
 // Named barriers between the warps of a tile: a barrier in shared memory takes its waiter 200 clocks beside warps that keep the
 // exponential unit busy, also when it is there already; a named one 30.  Every warp comes to all of its barriers, also after a wait
@@ -81,46 +81,6 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
     return all;
 }
 
-// The query rows of a CTA: up to `rows` tokens of sequence b from its token `first` on.
-struct ChBlock {
-    int b, first, len, row0, pos0;
-};
-
-// Block y counted from the last sequence's last block (the blocks with the most keys come first).  One warp.
-__device__ __forceinline__ ChBlock chunk_block(const Chunk& p, int y, int rows, int lane)
-{
-    int base = 0;
-    for (int i0 = 0; i0 < p.batch; i0 += 32) {
-        const int b = p.batch - 1 - (i0 + lane);
-        int lo = 0, len = 0;
-        if (b >= 0) {
-            lo = min(max(p.row_starts[b], 0), p.tokens);
-            len = min(max(p.row_starts[b + 1], lo), p.tokens) - lo;
-        }
-        const int n = (len + rows - 1) / rows;
-        int upto = n;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, upto, d);
-            if (lane >= d) upto += o;
-        }
-        const int total = __shfl_sync(0xffffffffu, upto, 31);
-        if (y < base + total) {
-            const int at = y - base;
-            const int from = __ffs(__ballot_sync(0xffffffffu, at < upto)) - 1;   // the first lane whose blocks reach so far
-            ChBlock r;
-            r.b = __shfl_sync(0xffffffffu, b, from);
-            r.len = __shfl_sync(0xffffffffu, len, from);
-            r.row0 = __shfl_sync(0xffffffffu, lo, from);
-            r.first = (__shfl_sync(0xffffffffu, upto, from) - 1 - at) * rows;
-            r.pos0 = p.positions[r.b];
-            return r;
-        }
-        base += total;
-    }
-    return ChBlock{-1, 0, 0, 0, 0};
-}
-
 template <int kTiles, int kUnits>
 __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 ? 2 : 1)
     attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
@@ -136,7 +96,6 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     uint64_t* drained = s_full + kTiles * 2;                                // [tiles]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    ChBlock* block_s = reinterpret_cast<ChBlock*>(tmem_slot + 2);
 
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int group = p.q_heads / p.kv_heads, tile_tokens = kChRows / group;
@@ -155,15 +114,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     }
     pdl_launch_dependents();
     pdl_wait();   // queries, cache rows and lists come from the kernels before this one
-    if (warp == S::load_warp) {
-        const ChBlock found = chunk_block(p, y, tile_tokens * kTiles, lane);
-        if (lane == 0) *block_s = found;
-    }
+    const ChunkBlock blk = p.blocks[y];
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const ChBlock blk = *block_s;
     if (blk.b < 0) {   // no rows for this CTA, and none for the others of its cluster
         if (warp == S::load_warp) tmem_dealloc(tmem_base, S::cols);
         return;
@@ -212,7 +167,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                         logical[u] += step_pages, within[u] += step_rest;
                         if (within[u] >= p.page_size) within[u] -= p.page_size, ++logical[u];
                     }
-                    page[u] = round < kChRounds && j < most_steps && pos < most ? __ldg(table + logical[u]) : -1;
+                    page[u] = round < kChRounds && j < most_steps && pos < most ? table[logical[u]] : -1;
                 }
             };
             const size_t row_bytes = size_t(p.kv_heads) * kChDim * 2;
@@ -563,12 +518,10 @@ int launch(const Chunk& p, int splits, cudaStream_t stream)
     if (int rc = make_tensor_map_2d_16bit(&q_map, p.queries, uint64_t(p.tokens) * p.q_heads, kChDim, kChRows)) return rc;
     const auto kernel = attn_chunk_tc_kernel<kTiles, kUnits>;
     GB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::total));
-    // blocks of a sequence's rows: ceil(rows / block) summed over the sequences, of whose lengths the host knows the sum's limit only
-    const int rows = kChRows / (p.q_heads / p.kv_heads) * kTiles;
-    const long long blocks = std::min<long long>(p.tokens, (long long)p.tokens / rows + p.batch);
-    if (blocks * p.kv_heads * splits > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: too many blocks of rows");
+    const long long ctas = (long long)p.block_count * p.kv_heads * splits;
+    if (ctas > 0x7fffffffll) return fail(GARNET_B200_NOT_SUPPORTED, "attention_chunk: too many blocks of rows");
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(blocks * p.kv_heads * splits));
+    cfg.gridDim = dim3(unsigned(ctas));
     cfg.blockDim = dim3(S::threads);
     cfg.dynamicSmemBytes = S::total;
     cfg.stream = stream;
@@ -585,9 +538,8 @@ int launch(const Chunk& p, int splits, cudaStream_t stream)
 
 }  // namespace
 
-int chunk_attention_launch(const Chunk& p, cudaStream_t stream)
+int chunk_attention_launch(const Chunk& p, const ChunkPlan& plan, cudaStream_t stream)
 {
-    const ChunkPlan plan = chunk_plan(p.batch, p.kv_heads, p.tokens, kChRows / (p.q_heads / p.kv_heads), p.max_context);
     if (plan.tiles == 2) return launch<2, 5>(p, plan.splits, stream);
     return plan.units == 2 ? launch<1, 2>(p, plan.splits, stream) : launch<1, 6>(p, plan.splits, stream);
 }

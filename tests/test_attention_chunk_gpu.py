@@ -170,6 +170,14 @@ def test_many_sequences():
     Case(lens, [int(n) for n in r.randint(0, 150, 70)], 4, 2).check()
 
 
+def test_more_sequences_than_threads_order_them():
+    """Blocks of rows are ordered by what they see: 600 sequences, many without rows, two of many blocks, in a buffer with room to spare."""
+    r = np.random.RandomState(1)
+    lens = [int(n) for n in r.randint(0, 4, 600)]
+    lens[17], lens[598], lens[599] = 700, 90, 1
+    Case(lens, [int(n) for n in r.randint(0, 60, 600)], 8, 1, pad=5).check()
+
+
 @pytest.mark.parametrize("q_heads,kv_heads,lens,starts,page_size", [
     (16, 8, [130, 90, 1, 127, 128, 129, 64, 65, 260, 0, 33, 100, 77, 128], [0, 5, 300, 128, 127, 1, 64, 63, 0, 9, 500, 250, 1, 0], 16),
     (18, 6, [90, 43, 85, 130, 84, 42, 41, 100, 100, 86, 129, 60, 70, 127, 3, 1, 88, 99, 47, 90], [20 * i for i in range(20)], 20),
