@@ -35,11 +35,11 @@ __device__ __forceinline__ uint32_t narrow(uint64_t v)
 // 20 of 10^6 by plain fp32 steps).
 // Bound: HBM in principle, the rows in and q, k and v out; in practice its instructions, some 250 for four heads with two values to an
 // instruction.
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 
 // One CTA beside the rows': the attention's blocks of rows by the keys that they see, the most first, so that the last CTAs to start
-// are short ones (24 ragged sequences of 5 rows at up to 3500: 47 instead of 65 us, a ragged batch of 8 prompts 58 instead of 74 us with
-// the sequences in their own order).  A counting sort; blocks that see equally much (within 1 / 1023 of max_context) come in any order.
+// are short ones (24 ragged sequences of 5 rows at up to 3500: 45 instead of 65 us, a ragged batch of 8 prompts 58 instead of 74 us with
+// the sequences in their own order).  A counting sort; blocks that see equally much (within 1 / 511 of max_context) come in any order.
 constexpr int kOrderBuckets = 4 * kRowThreads;
 __device__ __forceinline__ void chunk_order(const Chunk& p)
 {
@@ -97,7 +97,7 @@ __device__ __forceinline__ void chunk_order(const Chunk& p)
     for (int i = all + int(threadIdx.x); i < p.block_count; i += kRowThreads) p.blocks[i].b = -1;
 }
 
-__global__ void __launch_bounds__(kRowThreads, 4) attn_chunk_rows_kernel(const Chunk p, const int early)
+__global__ void __launch_bounds__(kRowThreads, 8) attn_chunk_rows_kernel(const Chunk p, const int early)
 {
     // few rows: the attention's CTAs come up beside these; many: they would only take their place
     if (early) pdl_launch_dependents();
@@ -278,7 +278,7 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = (flags & 1u) ? 1 : 0;
-    GB_CUDA(cudaLaunchKernelEx(&cfg, attn_chunk_rows_kernel, p, int(ctas <= 2 * kSmCount)));
+    GB_CUDA(cudaLaunchKernelEx(&cfg, attn_chunk_rows_kernel, p, int(ctas <= 4 * kSmCount)));
     return chunk_attention_launch(p, plan, s);
 }
 
