@@ -65,7 +65,7 @@ inline int oss_prefill_tiles(int batch, int kv_heads, int tokens, int tile_token
 // and the shares with the least estimated time are taken, the time being waves x (fixed part + steps x step), with figures
 // measured on a B200: a step of 64 keys takes 0.95, 0.74 and 0.9 us (1.3 us when two CTAs share the SM), the fixed part is 8, 6 and
 // 5 us, shares add 3 us.  Over 23 shapes from 1 to 8192 tokens at 0 to 30000 earlier ones, against the best of 12 plans each, it
-// takes 1.02 times as long on average and 1.18 at worst (64 ragged sequences of up to 4 tokens at up to 4000: 87 us, 74 in two shares).
+// takes 1.01 times as long on average and 1.12 at worst (24 equal sequences of one token at 3500: 88 us, 79 in four shares).
 // The plainer rule of two tiles where every SM then has a CTA, and otherwise one tile and shares for twice the SMs, took 162 instead
 // of 138 us for 512 tokens at 30000, and 34 instead of 24 us for 4 x 5 tokens at 4000.
 struct ChunkPlan {

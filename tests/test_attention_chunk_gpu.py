@@ -312,6 +312,29 @@ def test_same_bits_every_time_captured_and_on_another_stream():
         assert torch.equal(e["out"], first["out"])
 
 
+def test_calls_one_after_the_other_share_a_workspace():
+    """Launched without a wait between them, each starting while the one before ends, as the layers of a step are."""
+    cases = [Case([5, 9], [700, 30], 4, 2, seed=1), Case([150, 1], [0, 400], 4, 2, seed=2), Case([1, 1], [63, 64], 4, 2, seed=3)]
+    alone = [c.run()["out"] for c in cases]
+    shared = max(cases, key=lambda c: c.rows)
+    op = dec.ChunkAttention(shared.cfg, 160, 4096, 256, 4096)
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(4096, 128, shared.cfg.rope_theta))
+    given = []
+    for c in cases:
+        d = c.device()
+        table = torch.full((c.batch, 256), -1, dtype=torch.int32, device="cuda")
+        table[:, :c.width] = d["page_tables"]
+        given.append(dict(d, cos=cos, sin=sin, page_tables=table))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for d in given:
+            op.run(**d, pdl=True)
+    torch.cuda.synchronize()
+    for d, want in zip(given, alone):
+        off = (d["out"].double() - want.double()).norm()
+        assert off <= 2.0 ** -8 * want.double().norm()     # the keys may be shared out otherwise: P's rounding, the result's own
+
+
 def test_piece_after_piece_is_the_whole_prompt():
     """A prompt in one call, and in three pieces of odd lengths: the same keys and values, results within the two calls' roundings."""
     c = Case([300], [0], 4, 2, seed=10)
