@@ -19,10 +19,10 @@
 // Bound: a step of two tiles costs 1024 clocks of the exponential unit (16 per clock) and 1330 of the tensor pipe (N = 64 takes 50
 // clocks per MMA instead of 33: both operands come from shared memory); it takes 1800 (0.95 us): scores -> maximum -> exponentials
 // (780 clocks a tile, one tile after the other) -> P V is a chain.  B200, 16 / 8 heads, norms and cache append included: a prompt of
-// 8192 tokens 284 us (0.58 of the measured bf16 peak over the visible pairs), 512 tokens at 30000 132 us (0.58), a prompt of 2048
-// 45 us, 24 x 5 tokens at up to 3500 65 us (0.46 of the measured bandwidth), 4 tokens at 1000 10.8 us.  Steps of 128 keys with one
+// 8192 tokens 274 us (0.60 of the measured bf16 peak over the visible pairs), 512 tokens at 30000 128 us (0.60), a prompt of 2048
+// 42 us, 24 x 5 tokens at up to 3500 45 us (0.65 of the measured bandwidth), 4 tokens at 1000 10.0 us.  Steps of 128 keys with one
 // set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192 registers to a softmax thread) took 293 to 300 us
-// for 8192 tokens; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
+// for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
 // Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  P is rounded to bf16 where it meets V, 2^-8 of each
 // weight at most: the errors of the weights are independent of one another, so that a result is off by about what its own rounding
 // to bf16 takes (P in two pieces would cost half as many MMAs again).  A row that comes out NaN (infinities in places that it does not
