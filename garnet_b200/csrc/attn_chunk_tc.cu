@@ -398,12 +398,13 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         // a wait that gave up leaves NaNs, which no caller can take for a result
         const bool good = !*abort_flag;
         if (!good) sum = NAN;
+        const bool used = __any_sync(0xffffffffu, mine);
         if (splits == 1) {
             const float inv = end == 0 || sum == 0.f ? 0.f : 1.f / sum;
             __nv_bfloat16* out = p.out + (size_t(blk.row0 + t) * p.q_heads + head) * kChDim;
             bool bad = false;
 #pragma unroll 1
-            for (int c = 0; c < kChDim / 32; ++c) {
+            for (int c = 0; used && c < kChDim / 32; ++c) {
                 uint32_t o[32];
                 if (my_steps) {
                     tmem_ld_32x32(tm + S::col_o + 32 * c, o);
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
             const int i = q * kChRows + r, at = i / splits * splits + split;
             uint8_t* there = reinterpret_cast<uint8_t*>(cluster.map_shared_rank(smem, i % splits));
 #pragma unroll 1
-            for (int c = 0; c < kChDim / 32; ++c) {
+            for (int c = 0; used && c < kChDim / 32; ++c) {
                 uint32_t o[32];
                 if (my_steps) {
                     tmem_ld_32x32(tm + S::col_o + 32 * c, o);
@@ -456,7 +457,9 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         cluster.sync();
         // ---- this CTA's rows from the parts of all: four rows to a warp, eight lanes each
         constexpr int kWarps = S::threads / 32;
-        const int most_rows = (kTiles * kChRows - split + splits - 1) / splits, l = lane & 7;
+        // rows of the tiles up to the last that is a token's
+        const int tokens = blk.len - blk.first, used = kTiles == 2 && tokens > tile_tokens ? kChRows + min(tokens - tile_tokens, tile_tokens) * group : min(tokens, tile_tokens) * group;
+        const int most_rows = (used - split + splits - 1) / splits, l = lane & 7;
         for (int base = warp * 4; base < most_rows; base += kWarps * 4) {
             const int local = min(base + (lane >> 3), most_rows - 1), i = local * splits + split;
             const int q = i / kChRows, r = i % kChRows, in_tile = r / group, t = blk.first + q * tile_tokens + in_tile, head = kv * group + r % group;
