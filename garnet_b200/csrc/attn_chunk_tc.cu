@@ -19,7 +19,7 @@
 // Bound: a step of two tiles costs 1024 clocks of the exponential unit (16 per clock) and 1330 of the tensor pipe (N = 64 takes 50
 // clocks per MMA instead of 33: both operands come from shared memory); it takes 1800 (0.95 us): scores -> maximum -> exponentials
 // (780 clocks a tile, one tile after the other) -> P V is a chain.  B200, 16 / 8 heads, norms and cache append included: a prompt of
-// 8192 tokens 274 us (0.60 of the measured bf16 peak over the visible pairs), 512 tokens at 30000 128 us (0.60), a prompt of 2048
+// 8192 tokens 272 us (0.61 of the measured bf16 peak over the visible pairs), 512 tokens at 30000 128 us (0.60), a prompt of 2048
 // 42 us, 24 x 5 tokens at up to 3500 45 us (0.65 of the measured bandwidth), 4 tokens at 1000 10.0 us.  Steps of 128 keys with one
 // set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192 registers to a softmax thread) took 293 to 300 us
 // for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
