@@ -31,6 +31,7 @@
 #include <cooperative_groups.h>
 
 #include "attn_chunk.cuh"
+#include "chunk_barriers.h"
 #include "tc_common.cuh"
 
 namespace gb200 {
@@ -42,8 +43,8 @@ namespace cg = cooperative_groups;
 constexpr int kChRows = kChTileRows;   // query rows of a tile (UMMA M, one softmax thread each)
 constexpr int kChMaxSplits = 8;
 // Named barriers between the warps of a tile: a barrier in shared memory takes its waiter 200 clocks beside warps that keep the
-// exponential unit busy, also when it is there already; a named one 30.  Every warp comes to all of its barriers, also after a wait
-// that gave up.
+// exponential unit busy, also when it is there already; a named one 30.  Every warp comes to all of its barriers, in the order of
+// chunk_barriers.h, also after a wait that gave up.
 constexpr int kBarTurn = 1, kBarScores = 3, kBarP = 7;
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -234,12 +235,14 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
         bool good = true;
-        for (int i = 0; my_steps && i < my_steps + 2; ++i) {
-            good = good && wait_warp(&s_full[q * 2 + (i & 1)], (i >> 1) & 1, abort_flag);
-            tc_fence_after();
-            tc_fence_before();
-            bar_arrive(kBarScores + q * 2 + (i & 1), 160);
-        }
+        chunk_scout(
+            my_steps, [&](int i) { bar_sync(kBarP + q * 2 + (i & 1), kWeightsThreads); },
+            [&](int i) { good = good && wait_warp(&s_full[q * 2 + (i & 1)], (i >> 1) & 1, abort_flag); },
+            [&](int i) {
+                tc_fence_after();
+                tc_fence_before();
+                bar_arrive(kBarScores + q * 2 + (i & 1), kScoresThreads);
+            });
     } else if (warp >= S::mma_warp) {
         // ------------------------------------------- MMA issuers, one per tile
         constexpr uint32_t idesc_qk = umma_idesc_f16(1, kChRows, kKeys);
@@ -259,7 +262,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
             const uint32_t set = (u & 1) * kKeys;
             good = good && wait_warp(&full[unit], parity, abort_flag);
             const bool pv = u >= 2 && u < my_steps + 2;
-            if (pv) bar_sync(kBarP + q * 2 + (u & 1), 160);
+            if (pv) bar_sync(kBarP + q * 2 + (u & 1), kWeightsThreads);
             if (good && elect_one()) {
                 tc_fence_after();
                 if (pv) {
@@ -298,7 +301,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
         // the scores of step i, and with them P V of step i - 2; behind the last steps that alone
-        const auto scores_of = [&](int i) { bar_sync(kBarScores + q * 2 + (i & 1), 160); };
+        const auto scores_of = [&](int i) { bar_sync(kBarScores + q * 2 + (i & 1), kScoresThreads); };
         constexpr float kScale = 0.08838834764831845f * 1.4426950408889634f;   // 1 / sqrt(128), in powers of two
         float ref = -INFINITY, sum = 0.f;                                      // what the exponents are taken against; the weights' sum
         // steps in which the tiles take turns with their exponentials: left alone they fall into step, first both on the exponential
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
             if (!any) {   // none of the warp's rows sees a key: their weights may be what they are
                 if (j < turns && (q == 1 || j > 0)) bar_sync(kBarTurn + q, 256);
                 if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
-                bar_arrive(kBarP + q * 2 + (j & 1), 160);
+                bar_arrive(kBarP + q * 2 + (j & 1), kWeightsThreads);
                 continue;
             }
             tc_fence_after();
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
             if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
             tmem_st_wait();
             tc_fence_before();
-            bar_arrive(kBarP + q * 2 + (j & 1), 160);
+            bar_arrive(kBarP + q * 2 + (j & 1), kWeightsThreads);
             float part[2];
             f32x2_split(add2(part2[0], part2[1]), part[0], part[1]);
             sum += part[0] + part[1];
