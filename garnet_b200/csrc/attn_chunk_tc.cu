@@ -10,7 +10,7 @@
 //   MMA warps       one thread per tile: P V of step u - 2, then the scores of step u into the set that its P leaves;
 //   scout warps     one per tile: wait for the MMAs' barrier in shared memory and pass it on to a named one;
 //   softmax warps   one thread per query row: scores into registers, running maximum, p = 2^(s c - m c), the row's sum in fp32, P as
-//                   bf16 over the scores in tensor memory; O stays in tensor memory and is rescaled only when a row's maximum has
+//                   two bf16 numbers each over the scores in tensor memory; O stays in tensor memory and is rescaled only when a row's maximum has
 //                   grown by more than 2^8 since the last time (the final division makes that exact).  The fp32 work runs two
 //                   values per instruction.  Two tiles take turns with their exponentials.
 // Few rows after a long context: a cluster of up to 8 CTAs shares the keys; every CTA sends its part of row i to CTA i % splits by
@@ -23,10 +23,10 @@
 // 42 us, 24 x 5 tokens at up to 3500 45 us (0.65 of the measured bandwidth), 4 tokens at 1000 10.0 us.  Steps of 128 keys with one
 // set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192 registers to a softmax thread) took 293 to 300 us
 // for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
-// Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  P is rounded to bf16 where it meets V, 2^-8 of each
-// weight at most: the errors of the weights are independent of one another, so that a result is off by about what its own rounding
-// to bf16 takes (P in two pieces would cost half as many MMAs again).  A row that comes out NaN (infinities in places that it does not
-// see meet weights of zero) is computed again by the row loop.
+// Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  A weight of P meets V as two bf16 numbers, its
+// rounding and what that left out: 16 of its bits, 2^-16 of it at most lost, where one number (half as many MMAs of P V: 315 instead
+// of 383 us a call of 8192 rows) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places
+// that it does not see meet weights of zero) is computed again by the row loop.
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -50,6 +50,7 @@ __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("ba
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int kKeys = 64;         // keys of a step (UMMA N of Q K^T, K of P V)
 constexpr int kChRounds = kKeys / 32;   // P is handed over, and rows are copied, 32 keys at a time
+constexpr int kPieces = 2;        // bf16 numbers that a weight of P enters P V as
 constexpr int kChExists = 16;     // steps whose key bits are kept
 
 template <int kTiles, int kUnits>
@@ -269,7 +270,9 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                     const uint32_t v = v_lo + unit * (S::unit >> 4);
 #pragma unroll
                     for (int k16 = 0; k16 < kKeys / 16; ++k16)
-                        umma_f16_ts(tile + S::col_o, tile + set + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, u > 2 || k16 > 0);
+#pragma unroll
+                        for (int piece = 0; piece < kPieces; ++piece)
+                            umma_f16_ts(tile + S::col_o, tile + set + piece * (kKeys / 2) + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, u > 2 || k16 + piece > 0);
                 }
                 if (u < my_steps) {
                     const uint32_t k = k_lo + unit * (S::unit >> 4);
@@ -372,21 +375,25 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                 }
             }
             const float base = ref == -INFINITY ? 0.f : ref;
-            const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base);
+            const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base), minus1 = f32x2(-1.f, -1.f);
             uint64_t part2[2] = {0, 0};
             if (j < turns && (q == 1 || j > 0)) bar_sync(kBarTurn + q, 256);
 #pragma unroll
             for (int c = 0; c < kChRounds; ++c) {
-                uint32_t w[16];
+                uint32_t w[16], rest[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float a, d;
                     f32x2_split(fma2(f32x2(__uint_as_float(s[c][2 * i]), __uint_as_float(s[c][2 * i + 1])), scale2, base2), a, d);
-                    a = ex2(a), d = ex2(d);
-                    part2[i & 1] = add2(part2[i & 1], f32x2(a, d));
+                    const uint64_t both = f32x2(ex2(a), ex2(d));
+                    part2[i & 1] = add2(part2[i & 1], both);
+                    f32x2_split(both, a, d);
                     w[i] = bf16x2_of(a, d);
+                    f32x2_split(fma2(f32x2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), minus1, both), a, d);
+                    rest[i] = bf16x2_of(a, d);
                 }
                 tmem_st_32x16(ts + 16 * c, w);
+                tmem_st_32x16(ts + kKeys / 2 + 16 * c, rest);
             }
             if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
             tmem_st_wait();
