@@ -45,6 +45,7 @@ __device__ __forceinline__ void chunk_order(const Chunk& p)
 {
     __shared__ int places[kOrderBuckets], sums[kRowThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x < (kChSumSlots + 31) / 32) p.sum_slots[threadIdx.x] = 0;   // beside it: nobody holds a slot yet
     for (int i = threadIdx.x; i < kOrderBuckets; i += kRowThreads) places[i] = 0;
     __syncthreads();
     const auto every_block = [&](auto&& take) {   // take(block, its bucket)
@@ -208,9 +209,19 @@ int validate_chunk(const garnet_b200_attention_options* o)
     return GARNET_B200_OK;
 }
 
-// queries, and a block's entry per row at most
-size_t chunk_queries(const garnet_b200_attention_options& o, int tokens) { return size_t(tokens) * o.q_heads * kChDim * 2; }
-size_t chunk_workspace(const garnet_b200_attention_options& o, int tokens) { return chunk_queries(o, tokens) + size_t(tokens) * sizeof(ChunkBlock); }
+// The workspace: queries, a block's entry per row at most, the slots' bits, and sums where a context is long enough for them.
+struct ChunkSpace {
+    size_t blocks, slots, sums, bytes;
+};
+ChunkSpace chunk_space(const garnet_b200_attention_options& o, int tokens)
+{
+    ChunkSpace s;
+    s.blocks = size_t(tokens) * o.q_heads * kChDim * 2;
+    s.slots = s.blocks + size_t(tokens) * sizeof(ChunkBlock);
+    s.sums = (s.slots + (kChSumSlots + 31) / 32 * 4 + 255) & ~size_t(255);
+    s.bytes = s.sums + (o.max_context > kChSumSteps * 64 ? kChSumSlots * kChSumBytes : 0);
+    return s;
+}
 
 }  // namespace
 
@@ -224,7 +235,7 @@ int garnet_b200_attention_chunk_workspace(const garnet_b200_attention_options* o
 {
     if (int rc = validate_chunk(o)) return rc;
     if (!bytes || tokens <= 0) return fail(GARNET_B200_INVALID_VALUE, "attention_chunk_workspace: bad argument");
-    *bytes = chunk_workspace(*o, tokens);
+    *bytes = chunk_space(*o, tokens).bytes;
     return GARNET_B200_OK;
 }
 
@@ -238,9 +249,10 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     if (!d_qkv || !d_q_norm_weight || !d_k_norm_weight || !d_rope_cos || !d_rope_sin || !d_key_pages || !d_value_pages || !d_page_tables ||
         !d_positions || !d_row_starts || !d_out || batch <= 0 || tokens <= 0 || physical_pages <= 0)
         return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: null pointer, or batch, tokens or physical_pages not positive");
-    if (!d_workspace || workspace_bytes < chunk_workspace(*o, tokens) || (reinterpret_cast<uintptr_t>(d_workspace) & 255))
+    const ChunkSpace space = chunk_space(*o, tokens);
+    if (!d_workspace || workspace_bytes < space.bytes || (reinterpret_cast<uintptr_t>(d_workspace) & 255))
         return fail(GARNET_B200_INVALID_VALUE, "attention_chunk: the workspace is missing, too small (%zu < %zu) or not 256-byte aligned", workspace_bytes,
-                    chunk_workspace(*o, tokens));
+                    space.bytes);
     if ((reinterpret_cast<uintptr_t>(d_qkv) | reinterpret_cast<uintptr_t>(d_key_pages) | reinterpret_cast<uintptr_t>(d_value_pages) |
          reinterpret_cast<uintptr_t>(d_out) | reinterpret_cast<uintptr_t>(d_rope_cos) | reinterpret_cast<uintptr_t>(d_rope_sin) |
          reinterpret_cast<uintptr_t>(d_q_norm_weight) | reinterpret_cast<uintptr_t>(d_k_norm_weight)) & 15)
@@ -256,8 +268,11 @@ int garnet_b200_attention_chunk(const garnet_b200_attention_options* o, const vo
     p.values = static_cast<__nv_bfloat16*>(d_value_pages);
     p.tables = d_page_tables, p.positions = d_positions, p.row_starts = d_row_starts;
     p.out = static_cast<__nv_bfloat16*>(d_out);
-    p.queries = static_cast<__nv_bfloat16*>(d_workspace);
-    p.blocks = reinterpret_cast<ChunkBlock*>(static_cast<char*>(d_workspace) + chunk_queries(*o, tokens));
+    char* ws = static_cast<char*>(d_workspace);
+    p.queries = reinterpret_cast<__nv_bfloat16*>(ws);
+    p.blocks = reinterpret_cast<ChunkBlock*>(ws + space.blocks);
+    p.sum_slots = reinterpret_cast<unsigned*>(ws + space.slots);
+    p.sums = reinterpret_cast<float4*>(ws + space.sums);
     p.batch = batch, p.tokens = tokens, p.q_heads = o->q_heads, p.kv_heads = o->kv_heads, p.page_size = o->page_size;
     p.width = o->max_logical_pages, p.physical_pages = physical_pages, p.max_context = o->max_context;
     p.eps = o->norm_eps;

@@ -13,6 +13,14 @@ struct alignas(16) ChunkBlock {
     int b, first, len, row0, pos0, unused[3];
 };
 
+// Steps of 64 keys whose weights times values are added in the tensor core before the sum is added to those before in fp32.  The tensor
+// core cuts what it adds to a sum, eight times a step (16 keys to an MMA, two bf16 numbers to a weight), each time towards zero: sums of
+// positive terms lost 2^-28.5 of themselves per key and bf16 number, 2^-12.2 over 65536 keys and one number.  Sixty-four steps lose 2^-15.5,
+// a hundredth of the step between two results (8192 rows: 386 us a call with no such limit, 402 with 64 steps, 424 with 32).
+constexpr int kChSumSteps = 64;
+constexpr int kChSumSlots = 2 * kSmCount;                          // tiles that hold tensor memory at once: a tile has half of an SM's
+constexpr size_t kChSumBytes = size_t(kChTileRows) * kChDim * 4;   // a tile's sums
+
 struct Chunk {
     const __nv_bfloat16* qkv;        // [tokens, (q_heads + 2 kv_heads) * 128]
     const __nv_bfloat16* q_norm_w;   // [128]
@@ -27,6 +35,8 @@ struct Chunk {
     __nv_bfloat16* out;              // [tokens, q_heads * 128]
     __nv_bfloat16* queries;          // workspace: [kv head][token][q head of the group][128]
     ChunkBlock* blocks;              // workspace: the attention's blocks of rows, those that see the most keys first
+    unsigned* sum_slots;             // workspace: a bit for each of kChSumSlots, set while a tile holds it
+    float4* sums;                    // workspace: [slot][4 dims][row], where a context can be that long
     int batch, tokens, q_heads, kv_heads, page_size, width, physical_pages, max_context;
     int block_rows, block_count;     // tokens of a block; entries of `blocks`
     float eps;

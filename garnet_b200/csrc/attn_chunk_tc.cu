@@ -23,9 +23,11 @@
 // 42 us, 24 x 5 tokens at up to 3500 45 us (0.65 of the measured bandwidth), 4 tokens at 1000 10.0 us.  Steps of 128 keys with one
 // set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192 registers to a softmax thread) took 293 to 300 us
 // for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
-// Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  A weight of P meets V as two bf16 numbers, its
+// Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  The tensor core cuts towards zero what it adds to a
+// sum: O is taken out of tensor memory every kChSumSteps steps and added in fp32, in memory of the workspace (19 MB, which stay in L2)
+// of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its
 // rounding and what that left out: 16 of its bits, 2^-16 of it at most lost, where one number (half as many MMAs of P V: 315 instead
-// of 383 us a call of 8192 rows) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places
+// of 383 us a call of 8192 rows before sums were kept apart) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places
 // that it does not see meet weights of zero) is computed again by the row loop.
 #include <algorithm>
 #include <cooperative_groups.h>
@@ -75,6 +77,47 @@ struct ChShape {
     static_assert(kTiles * tile_cols <= 512, "tensor memory");
 };
 
+// A warp takes a slot, the first free one from `from` on: there are as many as there can be tiles that hold tensor memory, as this one
+// does.  (One that all want first takes the last of 256 tiles 15 us; looking at one after the other, 1 us each.)
+__device__ __noinline__ int take_slot(unsigned* bits, int from, int lane)
+{
+    constexpr int kWords = (kChSumSlots + 31) / 32;
+    static_assert(kWords <= 32, "a lane looks at a word");
+    const unsigned there = lane + 1 < kWords ? 0xffffffffu : lane + 1 == kWords ? 0xffffffffu >> (31 - (kChSumSlots - 1) % 32) : 0u;
+    for (int i = 0; i < 256; ++i) {
+        unsigned free = lane < kWords ? ~__ldcg(bits + lane) & there : 0u, behind = lane == from / 32 ? free & (0xffffffffu << (from & 31)) : lane > from / 32 ? free : 0u;
+        const unsigned words = __ballot_sync(0xffffffffu, behind != 0u), all = __ballot_sync(0xffffffffu, free != 0u);
+        if (!words) behind = free;
+        const int word = __ffs(words ? words : all) - 1;
+        int slot = -1;
+        if (lane == word) {
+            const unsigned bit = behind & (0u - behind);
+            if (!(atomicOr(bits + word, bit) & bit)) slot = word * 32 + __ffs(bit) - 1;
+            __threadfence();
+        }
+        slot = __shfl_sync(0xffffffffu, slot, max(word, 0));
+        if (word >= 0 && slot >= 0) return slot;
+    }
+    return -1;
+}
+
+// 32 dims of a row's kept sums; and o += f times them
+__device__ __forceinline__ void load_kept(const float4* from, float4 (&v)[8])
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __ldcg(from + i * kChRows);
+}
+__device__ __forceinline__ void add_kept(const float4 (&v)[8], float f, uint32_t (&o)[32])
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        o[4 * i] = __float_as_uint(fmaf(v[i].x, f, __uint_as_float(o[4 * i])));
+        o[4 * i + 1] = __float_as_uint(fmaf(v[i].y, f, __uint_as_float(o[4 * i + 1])));
+        o[4 * i + 2] = __float_as_uint(fmaf(v[i].z, f, __uint_as_float(o[4 * i + 2])));
+        o[4 * i + 3] = __float_as_uint(fmaf(v[i].w, f, __uint_as_float(o[4 * i + 3])));
+    }
+}
+
 // mbar_wait_warp without suspending: the softmax has its scores a hundred clocks sooner.
 __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort_flag)
 {
@@ -98,6 +141,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     uint64_t* drained = s_full + kTiles * 2;                                // [tiles]
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + kTiles);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile int* sum_slot = abort_flag + 1;                                // [tiles]: the tile's place in p.sums, -1 without one
 
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int group = p.q_heads / p.kv_heads, tile_tokens = kChRows / group;
@@ -108,6 +152,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         for (int i = 0; i < kTiles * 2; ++i) mbar_init(&s_full[i], 1);
         for (int q = 0; q < kTiles; ++q) mbar_init(&drained[q], 1);
         *abort_flag = 0;
+        for (int q = 0; q < kTiles; ++q) sum_slot[q] = -1;
         fence_barrier_init();
     }
     if (warp == S::load_warp) {
@@ -235,6 +280,12 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         int my_steps = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i) my_steps = i == q ? steps[i] : my_steps;
+        if (my_steps > kChSumSteps) {   // the softmax reads it behind the scores' barriers
+            const int taken = take_slot(p.sum_slots, int((blockIdx.x * kTiles + q) % kChSumSlots), lane);
+            sum_slot[q] = taken;
+            if (taken < 0) *abort_flag = 1;
+            __syncwarp();
+        }
         bool good = true;
         chunk_scout(
             my_steps, [&](int i) { bar_sync(kBarP + q * 2 + (i & 1), kWeightsThreads); },
@@ -272,7 +323,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                     for (int k16 = 0; k16 < kKeys / 16; ++k16)
 #pragma unroll
                         for (int piece = 0; piece < kPieces; ++piece)
-                            umma_f16_ts(tile + S::col_o, tile + set + piece * (kKeys / 2) + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, u > 2 || k16 + piece > 0);
+                            umma_f16_ts(tile + S::col_o, tile + set + piece * (kKeys / 2) + k16 * 8, v + k16 * (2048 >> 4), idesc_pv, (u - 2) % kChSumSteps != 0 || k16 + piece > 0);
                 }
                 if (u < my_steps) {
                     const uint32_t k = k_lo + unit * (S::unit >> 4);
@@ -311,6 +362,39 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         // unit, then neither
         const int turns = kTiles == 2 ? min(steps[0], steps[kTiles - 1]) : 0;
         const bool any = __any_sync(0xffffffffu, end > 0);
+        float kept = -INFINITY;   // what the weights of the kept sums stand against
+        const auto sums_of = [&] { return p.sums + size_t(sum_slot[q]) * (kChSumBytes / 16) + r; };
+        // O, the sum of up to kChSumSteps steps, is added to the steps' before; the next P V starts a sum of its own
+        const auto keep_sums = [&](int j) {
+            // O is complete when the scores of the next step are there
+            if (!*abort_flag) wait_warp(&s_full[q * 2 + ((j + 1) & 1)], ((j + 1) >> 1) & 1, abort_flag);
+            __syncwarp();
+            tc_fence_after();
+            if (sum_slot[q] < 0) return;   // and the call gives up
+            float4* to = sums_of();
+            const bool first = j == kChSumSteps, grown = __any_sync(0xffffffffu, kept != ref);
+            const float f = kept == ref ? 1.f : ex2(kept - ref);
+#pragma unroll 1
+            for (int c = 0; c < kChDim / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32(tm + S::col_o + 32 * c, o);
+                if (!first && grown) {   // seldom
+                    float4 v[8];
+                    load_kept(to + 8 * c * kChRows, v);
+                    tmem_ld_wait();
+                    add_kept(v, f, o);
+                }
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float4* at = to + (8 * c + i) * kChRows;
+                    const float4 v = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    if (first || grown) __stcg(at, v);
+                    else asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+                }
+            }
+            kept = ref;
+        };
         for (int j = 0; j < my_steps; ++j) {
             const int kb = (step0 + j) * kKeys;
             const uint32_t ts = tm + (j & 1) * kKeys;
@@ -397,6 +481,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
             }
             if (j < turns && !(q == 1 && j + 1 == turns)) bar_arrive(kBarTurn + 1 - q, 256);
             tmem_st_wait();
+            if (j > 0 && j % kChSumSteps == 0) keep_sums(j);
             tc_fence_before();
             bar_arrive(kBarP + q * 2 + (j & 1), kWeightsThreads);
             float part[2];
@@ -409,6 +494,19 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         const bool good = !*abort_flag;
         if (!good) sum = NAN;
         const bool used = __any_sync(0xffffffffu, mine);
+        // 32 dims of O, with what was kept
+        const float kept_scale = kept == ref ? 1.f : ex2(kept - ref);
+        const bool with_kept = my_steps > kChSumSteps && any && sum_slot[q] >= 0;
+        float4 next[8];   // a trip to L2 ahead
+        if (with_kept) load_kept(sums_of(), next);
+        const auto load_o = [&](int c, uint32_t (&o)[32]) {
+            tmem_ld_32x32(tm + S::col_o + 32 * c, o);
+            tmem_ld_wait();
+            if (with_kept) {
+                add_kept(next, kept_scale, o);
+                if (c + 1 < kChDim / 32) load_kept(sums_of() + 8 * (c + 1) * kChRows, next);
+            }
+        };
         if (splits == 1) {
             const float inv = end == 0 || sum == 0.f ? 0.f : 1.f / sum;
             __nv_bfloat16* out = p.out + (size_t(blk.row0 + t) * p.q_heads + head) * kChDim;
@@ -416,10 +514,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
 #pragma unroll 1
             for (int c = 0; used && c < kChDim / 32; ++c) {
                 uint32_t o[32];
-                if (my_steps) {
-                    tmem_ld_32x32(tm + S::col_o + 32 * c, o);
-                    tmem_ld_wait();
-                }
+                if (my_steps) load_o(c, o);
                 if (mine) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -448,10 +543,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
 #pragma unroll 1
             for (int c = 0; used && c < kChDim / 32; ++c) {
                 uint32_t o[32];
-                if (my_steps) {
-                    tmem_ld_32x32(tm + S::col_o + 32 * c, o);
-                    tmem_ld_wait();
-                }
+                if (my_steps) load_o(c, o);
                 if (mine) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
@@ -518,6 +610,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     tc_fence_before();
     __syncthreads();
     if (warp == S::load_warp) {
+        if (lane < kTiles && sum_slot[lane] >= 0) {   // nobody of this CTA reads or writes there any more
+            __threadfence();
+            atomicAnd(p.sum_slots + sum_slot[lane] / 32, ~(1u << (sum_slot[lane] & 31)));
+        }
+        __syncwarp();
         tc_fence_after();
         tmem_dealloc(tmem_base, S::cols);
     }

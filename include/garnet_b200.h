@@ -336,8 +336,9 @@ int garnet_b200_attention_decode(const garnet_b200_attention_options* options, c
  *   - What the cache holds behind a sequence's last slot does not matter (NaN and infinities included).
  *   - Pages that hold the slots of new rows belong to one sequence each; full pages before them may be shared.
  *   - q_heads / kv_heads at most 128.  Rows, cache pages, norm weights, rope tables and output start on 16-byte boundaries.
- * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned) needs no clearing and holds nothing
- * between calls; calls that overlap on the GPU need one each.  flags bit 0: programmatic dependent launch.  No allocation, no
+ * Weights enter their products with the values with 16 bits, all sums are fp32.
+ * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned; 19 MB of it for sums where max_context is
+ * above 4096) needs no clearing and holds nothing between calls; calls that overlap on the GPU need one each.  flags bit 0: programmatic dependent launch.  No allocation, no
  * synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step
  * (src/cuda/text_kv_attention_kernel.cu:640-840). */
 int garnet_b200_attention_chunk_workspace(const garnet_b200_attention_options* options, int tokens, size_t* bytes);

@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 import torch
 
+from garnet_b200 import decode as dec
 from test_attention_chunk_gpu import Case
 
 pytestmark = pytest.mark.gpu
@@ -24,3 +25,63 @@ def test_weights_keep_sixteen_bits(lens, starts, heads):
     off = np.abs(d["out"].double().cpu().numpy() - want)
     bad = off > 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * mass
     assert not bad.any(), f"{bad.sum()} of {bad.size}, the largest by {(off - 2.0 ** -8 * np.abs(want))[bad].max() / mass.max()}"
+
+
+@pytest.mark.parametrize("tokens,context,heads", [(1, 131072, 8), (2048, 32768, 16), (2048, 65536, 16), (9000, 9000, 8)])
+def test_long_sums_lose_no_more_than_short_ones(tokens, context, heads):
+    """Equal weights (queries of zeros) and positive values of many magnitudes: a tensor core that adds them all loses 2^-28.5 per key, in one
+    direction (12 of 1024 results were a step too low after 32768 keys).  Added in fp32 after every 64 steps of 64 keys, a sum loses 2^-23 of
+    itself per MMA of 256 at most, half of that on average over its growth: 2^-16.  A quarter of that again for all that follows: sums of up
+    to 32 parts and a division in fp32."""
+    gen = torch.Generator(device="cuda").manual_seed(tokens)
+    kv, pages = 8, context // 16 + 1
+    cfg = dec.DecoderConfig(q_heads=heads, kv_heads=kv)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(16 * pages, 128, cfg.rope_theta))
+    one = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    table = torch.randperm(pages, device="cuda", generator=gen).to(torch.int32)[None]
+    op = dec.ChunkAttention(cfg, tokens, 16 * pages, pages, 16 * pages)
+    for _ in range(3):
+        values = torch.exp2(-12 * torch.rand(16 * pages, kv, 128, device="cuda", generator=gen)).to(torch.bfloat16)
+        cache = torch.empty(pages, 16, kv, 128, dtype=torch.bfloat16, device="cuda")
+        cache[table[0].long()] = values.view(pages, 16, kv, 128)
+        qkv = torch.zeros(tokens, heads + 2 * kv, 128, dtype=torch.bfloat16, device="cuda")
+        qkv[:, heads + kv:] = values[context - tokens:context]
+        out = torch.zeros(tokens, heads * 128, dtype=torch.bfloat16, device="cuda")
+        op.run(qkv.view(tokens, -1), one, one, cos, sin, torch.zeros_like(cache), cache, table, ints(context - tokens), ints(0, tokens), out)
+        for row in {0, tokens // 2, tokens - 1}:
+            want = values[:context - tokens + row + 1].double().mean(0).repeat_interleave(heads // kv, 0)
+            got = out[row].view(heads, 128).double()
+            half_step = torch.exp2(torch.floor(torch.log2(want)) - 8)
+            over = ((got - want).abs() - half_step) / want
+            assert float(over.max()) <= 1.25 * 2.0 ** -16, f"row {row}: {int((over > 1.25 * 2.0 ** -16).sum())} of {over.numel()}, {float(over.max())}"
+
+
+def test_weights_and_sums_after_a_long_context():
+    """General weights, up to 41000 positions, pages missing; two tiles, one tile in shares."""
+    for lens, starts, heads in (([3], [41000], (2, 1)), ([1], [41000], (4, 4)), ([130], [7000], (4, 1))):
+        c = Case(lens, starts, *heads, seed=12)
+        c.table[0, 5::97] = -1
+        d = c.run()
+        want, tol, _, _ = c.expect()
+        mass = (tol - 2.0 ** -8 * np.abs(want)) / (2.0 ** -8 + 2.0 ** -11)
+        off = np.abs(d["out"].double().cpu().numpy() - want)
+        bad = off > 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * mass
+        assert not bad.any(), f"{bad.sum()} of {bad.size}"
+
+
+@pytest.mark.parametrize("lens,starts,heads", [([140], [9000], (2, 1)), ([1], [70000], (2, 1))])
+def test_maxima_that_grow_along_a_long_context(lens, starts, heads):
+    """Kept sums are scaled to larger and larger maxima.  Scores up to 2^6 in powers of two, products up to 2^9: cut eight times at 2^-15, 2^-15 in
+    the exponent, twice (result and denominator), beside what the others have: less than 2^-13 of the mass."""
+    c = Case(lens, starts, *heads, seed=13)
+    at = torch.arange(starts[0])
+    scale = 0.05 + 10 * at / starts[0]
+    pages, offsets = c.table[0, (at // 16).long()].long(), at % 16
+    c.keys[pages, offsets] = (c.keys[pages, offsets].float() * scale[:, None, None]).to(torch.bfloat16)
+    d = c.run()
+    want, tol, _, _ = c.expect()
+    mass = (tol - 2.0 ** -8 * np.abs(want)) / (2.0 ** -8 + 2.0 ** -11)
+    off = np.abs(d["out"].double().cpu().numpy() - want)
+    bad = off > 2.0 ** -8 * np.abs(want) + 2.0 ** -13 * mass
+    assert not bad.any(), f"{bad.sum()} of {bad.size}"
