@@ -7,7 +7,7 @@
 // turn: four 16-byte loads per lane, the block's maximum (NaN wins) by packed maxima and one warp reduction, which also says whether the
 // warp's reference has to grow (by more than 2^8, so that this is rare: S and W are rescaled then), then per value one conversion,
 // half of a packed multiply-add, one exponential and half of two packed additions; the rank is counted in packed 16-bit numbers,
-// in blocks whose maximum is above the target's logit.
+// in blocks whose maximum is above the target's logit or NaN.
 // The block maxima stay in shared memory.  The top_k-th largest of the threads' own maxima is no larger than the top_k-th
 // largest logit, so that only blocks that reach it - few more than top_k - are read a second time (from L2) for the alternatives: every
 // value that reaches it becomes a candidate, (value, lowest index) as one 64-bit number, and the candidates larger than it say its place.
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kLpThreads, 1024 / kLpThreads) log_probs_kerne
         lane_top = fmaxf(lane_top, m);   // a NaN loses
         asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(m));
         grow(m);
-        if (m > x_t) {   // else none of the block is larger than the target's; a row with a NaN needs no rank
+        if (!(m <= x_t)) {   // else none of the block is larger than the target's; beside a NaN there may be larger ones
 #pragma unroll
             for (int k = 0; k < kLpVecs; ++k) count.add(v[k]);
         }

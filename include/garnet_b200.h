@@ -364,8 +364,8 @@ int garnet_b200_argmax_bf16(const void* d_logits, int* d_out, int batch, int voc
  * when top_k is 0; top_k is at most 32 and at most vocab.
  *   - A target outside 0 .. vocab - 1 (a row without one) gets log probability 0 and rank 0.
  *   - Logits of -inf have probability 0 and add nothing; a row of nothing else has log probabilities -inf and entropy 0.
- *   - A NaN or +inf among a row's logits makes its log probabilities and entropy NaN.  NaN is no alternative: where a row has fewer than
- *     top_k others, the ids behind them are -1.
+ *   - A NaN or +inf among a row's logits makes its log probabilities and entropy NaN.  Ranks count the logits that are larger all the
+ *     same; nothing is larger than a NaN.  NaN is no alternative: where a row has fewer than top_k others, the ids behind them are -1.
  * Sums are fp32; no workspace, no allocation, no synchronisation; the results do not depend on timing.  flags bit 0: programmatic
  * dependent launch.  The reference's sampler stops at the top token (src/cuda/logits_sampler_kernel.cu). */
 int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, const int* d_targets, int rows, int vocab, int top_k,

@@ -143,6 +143,25 @@ def test_nan_and_infinity(rows_each):
         assert ids[i, 3].tolist() == [4, 900, -1, -1]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,offset", [(1, 0), (3, 5), (700, 3)])
+def test_ranks_beside_nan(dtype, rows, offset):
+    """The rank counts the larger logits of the whole row, wherever a NaN lies and however the row is cut into blocks and parts; nothing
+    is larger than a NaN."""
+    n = 20011
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    flat = torch.randn(rows * n + offset, device="cuda", generator=gen).to(dtype)
+    x = flat[offset:].view(rows, n)
+    nans = torch.randint(0, n, (rows, 3), device="cuda", generator=gen)
+    x.scatter_(1, nans, float("nan"))
+    targets = torch.randint(0, n, (rows,), dtype=torch.int32, device="cuda", generator=gen)
+    targets[rows // 2] = nans[rows // 2, 0]
+    r = dec.log_probs(x, targets, top_k=2)
+    want = (x > x.gather(1, targets.long()[:, None])).sum(1) + 1
+    assert torch.equal(r.ranks.long(), want) and int(r.ranks[rows // 2]) == 1
+    assert r.log_probs.isnan().all() and r.entropy.isnan().all()
+
+
 def test_without_targets_unaligned_and_many_rows():
     gen = torch.Generator(device="cuda").manual_seed(2)
     flat = torch.randn(70000 * 17 + 3, device="cuda", generator=gen).to(torch.bfloat16)
