@@ -60,7 +60,8 @@ class PagePool:
         return n
 
     def extend(self, sequences, tokens):
-        """sequences[i] grows by tokens[i] positions.  Returns a status per entry (0; 1: refused; 5: too few free pages)."""
+        """sequences[i] grows by tokens[i] positions.  Returns a status per entry (0; 1: refused; 5: too few free pages).  An entry that is not 0
+        changed nothing: where the sequence has no page for its next slot (-1), the attention calls append nothing and do not see that token."""
         n = self._entries(sequences, "sequences")
         self._list(tokens, "tokens", n)
         status = torch.empty(n, dtype=torch.int32, device=self.device)

@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attention_decode_kernel(const
         for (int u = 0; u < kPer; ++u) {
             const int pos = start + warp + u * kAttnWarps;
             const int pg = __shfl_sync(0xffffffffu, page, u);
-            if (pos < end && pos != slot) {
+            if (pos < end && pos != slot && pg >= 0) {
                 const size_t at = ((size_t(pg) * p.page_size + pos % p.page_size) * p.kv_heads + kv_head) * kAttnHeadDim;
                 cp_async_8(my_k + u * (kAttnHeadDim * 2) + lane * 8, reinterpret_cast<const uint2*>(p.key_pages + at) + lane);
                 cp_async_8(my_v + u * (kAttnHeadDim * 2) + lane * 8, reinterpret_cast<const uint2*>(p.value_pages + at) + lane);
@@ -146,13 +146,14 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attention_decode_kernel(const
         float o[4];
         norm_rope_head(row + q_width + kv_head * kAttnHeadDim, p.k_norm_w, cs, sn, p.eps, lane, o);
         const __nv_bfloat16* v_row = row + q_width + kv_width + kv_head * kAttnHeadDim;
-        const size_t at = ((size_t(table[slot / p.page_size]) * p.page_size + slot % p.page_size) * p.kv_heads + kv_head) * kAttnHeadDim;
+        const int pg = table[slot / p.page_size];
+        const size_t at = ((size_t(pg) * p.page_size + slot % p.page_size) * p.kv_heads + kv_head) * kAttnHeadDim;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = lane + 32 * i;
             k_new[d] = o[i];
             v_new[d] = __bfloat162float(v_row[d]);
-            if (q_head % group == 0) {   // one CTA per kv head appends to the cache
+            if (q_head % group == 0 && pg >= 0) {   // one CTA per kv head appends to the cache
                 p.key_pages[at + d] = __float2bfloat16_rn(o[i]);
                 p.value_pages[at + d] = v_row[d];
             }
@@ -172,6 +173,7 @@ __global__ void __launch_bounds__(kAttnWarps * 32) attention_decode_kernel(const
         for (int u = 0; u < kPer; ++u) {
             const int pos = start + warp + u * kAttnWarps;
             if (pos >= end) break;
+            if (__shfl_sync(0xffffffffu, page, u) < 0) continue;   // a slot without a page is not seen
             float kf[4], vf[4];
             if (pos == slot) {   // the new token's row is not read back from the cache
 #pragma unroll

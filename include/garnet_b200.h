@@ -319,6 +319,8 @@ int garnet_b200_attention_decode_workspace(const garnet_b200_attention_options* 
  *   k, v are written to the cache at ((page_table[b][slot / page_size] * page_size + slot % page_size)
  *          * kv_heads + kv_head) * 128 (the reference's layout, text_kv_attention_kernel.cu:668-673);
  *   out[b, h*128 ..] = softmax(q_h . K^T / sqrt(128)) V over the context, fp32 arithmetic, bf16 result.
+ * A slot whose page is negative (a row of the table that the pool left without one) is not written and not seen; a context of nothing
+ * else gives zeros.  Page numbers that are not negative are taken as they are: they must lie in the cache.
  * flags bit 0: programmatic dependent launch.  No allocation, no synchronisation. */
 int garnet_b200_attention_decode(const garnet_b200_attention_options* options, const void* d_qkv, const void* d_q_norm_weight,
                                  const void* d_k_norm_weight, const float* d_rope_cos, const float* d_rope_sin, void* d_key_pages,

@@ -426,3 +426,29 @@ def decode_only(decode, rows, qn, kn, cos, sin, keys, values, pool, i32):
     y = torch.zeros(4, 512, dtype=torch.bfloat16, device="cuda")
     decode.run(rows[63:64].repeat(4, 1), qn, kn, cos, sin, keys[0], values[0], pool.page_tables, i32(63, 63, 63, -1), y)
     return y
+
+
+def test_the_decode_kernel_and_pages_that_do_not_exist():
+    """garnet_b200_attention_decode on tables as PagePool leaves them: a slot without a page (-1) is neither written nor seen, a row that sees none is
+    zeros; nothing else in the cache changes."""
+    starts = [40, 300, 16, 129, 0, 255]
+    c = Case([1] * len(starts), starts, 4, 2, seed=21)
+    c.table[0, 1] = -1                               # a page of the context
+    c.table[1, 300 // 16] = -1                       # the page that the new token falls into: a pool that was full
+    c.table[2, 16 // 16] = -1
+    c.table[3, :8] = -1                              # a whole split of the context
+    c.table[4, :] = -1                               # a sequence without pages
+    c.table[5, :] = -7
+    want, tol, keys, values = c.expect()
+    d = c.device()
+    guard = [torch.full((c.pages + 2, *c.keys.shape[1:]), 3.0, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for g, name in zip(guard, ("key_pages", "value_pages")):
+        g[1:-1] = d[name]
+    attn = dec.PagedAttention(c.cfg, c.batch, c.max_context, c.width, c.positions_room)
+    for _ in range(2):
+        attn.run(d["qkv"], d["q_norm_w"], d["k_norm_w"], d["cos"], d["sin"], guard[0][1:-1], guard[1][1:-1], d["page_tables"], d["positions"], d["out"])
+        got = d["out"].double().cpu().numpy()
+        assert (np.abs(got - want) <= tol).all() and (got[4:] == 0).all()
+    assert all((g[0] == 3).all() and (g[-1] == 3).all() for g in guard)
+    assert np.array_equal(guard[1][1:-1].float().cpu().numpy(), values)
+    assert (np.abs(guard[0][1:-1].float().cpu().numpy() - keys) <= 2.0 ** -7 * np.abs(keys)).all()      # k by plain fp32 steps: a neighbour at most
