@@ -71,6 +71,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.garnet_b200_cache_fork.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, vp, sz, vp]
     L.garnet_b200_cache_free.argtypes = [vp, vp, vp, vp, vp, i, vp]
     L.garnet_b200_cache_compact.argtypes = [vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    L.garnet_b200_cache_compact_ex.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     L.garnet_b200_cache_copy_pages.argtypes = [vp, vp, vp, vp, vp, i, vp]
     L.garnet_b200_embedding_gather.argtypes = [vp, vp, vp, i, i, i, c.c_uint, vp]
     L.garnet_b200_argmax_bf16.argtypes = [vp, vp, i, i, c.c_uint, vp]

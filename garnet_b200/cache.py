@@ -86,13 +86,17 @@ class PagePool:
         if n:
             check(lib().garnet_b200_cache_free(self._opt, *self._state, sequences.data_ptr(), n, stream_ptr()))
 
-    def compact(self):
-        """Moves the live pages to the numbers 0 .. live - 1.  Returns live, a device tensor of one number."""
+    def compact(self, moved=None):
+        """Moves the live pages to the numbers 0 .. live - 1.  Returns live, a device tensor of one number.  `moved` (int32 [pages], on the
+        device) is given the new number of every page that was live, its own number where it stays: a page that is held by a count of the
+        caller's own, not by a table, is found by it."""
         live = torch.empty(1, dtype=torch.int32, device=self.device)
         if torch.cuda.current_device() != self.device.index:
             raise ValueError("the pool is on another device than the current one")
-        check(lib().garnet_b200_cache_compact(self._opt, self._k, self._v, self._state[0], self._state[2], live.data_ptr(), *self._work,
-                                              stream_ptr()))
+        if moved is not None:
+            self._list(moved, "moved", self.opt.physical_pages)
+        check(lib().garnet_b200_cache_compact_ex(self._opt, self._k, self._v, self._state[0], self._state[2], live.data_ptr(),
+                                                 None if moved is None else moved.data_ptr(), *self._work, stream_ptr()))
         return live
 
     def copy_pages(self, src, dst) -> None:

@@ -25,10 +25,10 @@
 // for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
 // Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  The tensor core cuts towards zero what it adds to a
 // sum: O is taken out of tensor memory every kChSumSteps steps and added in fp32, in memory of the workspace (19 MB, which stay in L2)
-// of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its
-// rounding and what that left out: 16 of its bits, 2^-16 of it at most lost, where one number (half as many MMAs of P V: 315 instead
-// of 383 us a call of 8192 rows before sums were kept apart) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places
-// that it does not see meet weights of zero) is computed again by the row loop.
+// of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its rounding and what that left out: 16 of its
+// bits, 2^-16 of it at most lost, where one number (half as many MMAs of P V: 315 instead of 383 us a call of 8192 rows before sums
+// were kept apart) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places that it does
+// not see meet weights of zero) is computed again by the row loop.
 #include <algorithm>
 #include <cooperative_groups.h>
 

@@ -55,8 +55,9 @@ struct PoolWork {
     int* page;        // [count]: fork: the new page, -1 where there is none
     int* ids;         // [physical pages]: free pages in order; compact: source pages of the moves
     int* dst;         // [physical pages]: compact: destinations of the moves
-    int* map;         // [physical pages]: compact: new number of a page
+    int* map;         // [physical pages]: compact: new number of a page, for those with the number `map_from` or more
     int* moves;       // [1]
+    int map_from;     // -1: the count of live pages
 };
 
 size_t align64(size_t n) { return (n + 63) & ~size_t(63); }
@@ -77,6 +78,7 @@ PoolWork pool_work(const garnet_b200_cache_options& o, int count, void* ws)
     w.first = take(size_t(count)), w.need = take(size_t(count)), w.page = take(size_t(count));
     w.ids = take(size_t(o.physical_pages)), w.dst = take(size_t(o.physical_pages)), w.map = take(size_t(o.physical_pages));
     w.moves = take(1);
+    w.map_from = -1;
     return w;
 }
 
@@ -333,7 +335,7 @@ __global__ void __launch_bounds__(kPlanThreads) pool_compact_plan_kernel(const P
     }
     list_pages(t.refs, from, below, true, w.dst, holes_before, moves);
     list_pages(t.refs, above, to, false, w.ids, movers_before, moves);
-    for (int p = live + int(threadIdx.x); p < t.physical_pages; p += kPlanThreads) w.map[p] = p;
+    for (int p = (w.map_from < 0 ? live : w.map_from) + int(threadIdx.x); p < t.physical_pages; p += kPlanThreads) w.map[p] = p;
     __syncthreads();
     for (int i = threadIdx.x; i < moves; i += kPlanThreads) {
         const int src = __ldcg(&w.ids[i]), dst = __ldcg(&w.dst[i]);
@@ -523,8 +525,8 @@ int garnet_b200_cache_free(const garnet_b200_cache_options* o, int* d_page_table
     return GARNET_B200_OK;
 }
 
-int garnet_b200_cache_compact(const garnet_b200_cache_options* o, void* const* key_pages, void* const* value_pages, int* d_page_tables,
-                              int* d_refcounts, int* d_live, void* d_workspace, size_t workspace_bytes, void* stream)
+int garnet_b200_cache_compact_ex(const garnet_b200_cache_options* o, void* const* key_pages, void* const* value_pages, int* d_page_tables,
+                                 int* d_refcounts, int* d_live, int* d_moved, void* d_workspace, size_t workspace_bytes, void* stream)
 {
     if (int rc = validate_cache(o)) return rc;
     if (!d_page_tables || !d_refcounts || !d_live) return fail(GARNET_B200_INVALID_VALUE, "cache_compact: null pointer");
@@ -532,12 +534,19 @@ int garnet_b200_cache_compact(const garnet_b200_cache_options* o, void* const* k
     if (int rc = pool_layers(*o, key_pages, value_pages, "cache_compact", &layers)) return rc;
     if (int rc = pool_check_ws(*o, 0, d_workspace, workspace_bytes, "cache_compact")) return rc;
     const PoolTables t = pool_tables(*o, d_page_tables, nullptr, d_refcounts);
-    const PoolWork w = pool_work(*o, 0, d_workspace);
+    PoolWork w = pool_work(*o, 0, d_workspace);
+    if (d_moved) w.map = d_moved, w.map_from = 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     pool_compact_plan_kernel<<<1, kPlanThreads, 0, s>>>(t, w, d_live);
     GB_CUDA(cudaGetLastError());
     GB_CUDA(launch_behind(pool_compact_kernel, dim3(unsigned(kCopyCtas)), s, layers, t, w, static_cast<const int*>(d_live)));
     return GARNET_B200_OK;
+}
+
+int garnet_b200_cache_compact(const garnet_b200_cache_options* o, void* const* key_pages, void* const* value_pages, int* d_page_tables,
+                              int* d_refcounts, int* d_live, void* d_workspace, size_t workspace_bytes, void* stream)
+{
+    return garnet_b200_cache_compact_ex(o, key_pages, value_pages, d_page_tables, d_refcounts, d_live, nullptr, d_workspace, workspace_bytes, stream);
 }
 
 int garnet_b200_cache_copy_pages(const garnet_b200_cache_options* o, void* const* key_pages, void* const* value_pages, const int* d_src,

@@ -340,8 +340,8 @@ int garnet_b200_attention_decode(const garnet_b200_attention_options* options, c
  *   - q_heads / kv_heads at most 128.  Rows, cache pages, norm weights, rope tables and output start on 16-byte boundaries.
  * Weights enter their products with the values with 16 bits, all sums are fp32.
  * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned; 19 MB of it for sums where max_context is
- * above 4096) needs no clearing and holds nothing between calls; calls that overlap on the GPU need one each.  flags bit 0: programmatic dependent launch.  No allocation, no
- * synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step
+ * above 4096) needs no clearing and holds nothing between calls; calls that overlap on the GPU need one each.  flags bit 0:
+ * programmatic dependent launch.  No allocation, no synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step
  * (src/cuda/text_kv_attention_kernel.cu:640-840). */
 int garnet_b200_attention_chunk_workspace(const garnet_b200_attention_options* options, int tokens, size_t* bytes);
 int garnet_b200_attention_chunk(const garnet_b200_attention_options* options, const void* d_qkv, const void* d_q_norm_weight,
@@ -380,8 +380,8 @@ int garnet_b200_log_probs(const void* d_logits, int dtype, int64_t row_stride, c
  * that the caller owns: d_page_tables [sequences, max_logical_pages] (what the attention calls read; -1 where a row has no page),
  * d_lengths [sequences] (positions that a sequence holds, in its first ceil(length / page_size) pages) and
  * d_refcounts [physical_pages] (table entries that refer to the page; 0 = free).  An empty pool is -1, 0 and 0.  A host that pins a
- * page adds one to its count.  Lists (sequence numbers, token counts, pages) are int32 arrays on the device.  The outcome is a
- * function of state and lists alone.  d_status[i]: GARNET_B200_OK, _INVALID_VALUE (entry i is refused) or _OUT_OF_MEMORY (too few free
+ * page adds one to its count, and follows the page through garnet_b200_cache_compact_ex when the pool is moved together.  Lists
+ * (sequence numbers, token counts, pages) are int32 arrays on the device.  The outcome is a function of state and lists alone.  d_status[i]: GARNET_B200_OK, _INVALID_VALUE (entry i is refused) or _OUT_OF_MEMORY (too few free
  * pages: from the first entry on that does not get its pages, entries that need one get none; nothing is changed for them).
  * key_pages / value_pages are host arrays of `layers` device pointers (16-byte aligned, read during the call), the cache of each layer
  * [physical_pages][page_size][token_bytes].  Calls on one pool are ordered by their stream.  The workspace
@@ -416,6 +416,11 @@ int garnet_b200_cache_free(const garnet_b200_cache_options* options, int* d_page
  * of `live` or more goes to the i-th free page below it; tables and counts follow.  d_live[0] = live. */
 int garnet_b200_cache_compact(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages, int* d_page_tables,
                               int* d_refcounts, int* d_live, void* d_workspace, size_t workspace_bytes, void* stream);
+/* The same, with the page numbers' change in d_moved [physical_pages] (NULL: not asked for): the new number of every page that was live, its
+ * own number where it stays and for pages that were free.  A host that refers to pages by itself (pins) has to follow it. */
+int garnet_b200_cache_compact_ex(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages,
+                                 int* d_page_tables, int* d_refcounts, int* d_live, int* d_moved, void* d_workspace, size_t workspace_bytes,
+                                 void* stream);
 /* Copies page d_src[i] to page d_dst[i] in every layer, as if one pair after the other; pairs with a page outside the cache are passed over. */
 int garnet_b200_cache_copy_pages(const garnet_b200_cache_options* options, void* const* key_pages, void* const* value_pages, const int* d_src,
                                  const int* d_dst, int count, void* stream);

@@ -262,6 +262,44 @@ def test_pages_behind_two_gigabytes():
     assert torch.equal(keys[0, 0], want_k)
 
 
+def test_pages_that_the_host_holds_are_found_again():
+    """Pages whose only reference is a count of the host's: moved together with the others, found by `moved`, not handed out, given back."""
+    pool, keys, values, model = make(2, 40, 4, 1, 64, 6, 20)
+    seqs = [0, 1, 2, 3]
+    assert pool.extend(ints(seqs), ints([30, 25, 17, 40])).tolist() == model.extend(seqs, [30, 25, 17, 40])
+    pinned = [int(model.table[1, 0]), int(model.table[2, 4]), int(model.table[3, 9])]
+    for p in pinned:
+        pool.refcounts[p] += 1
+        model.refs[p] += 1
+    held = [[t[p].clone() for t in (*keys, *values)] for p in pinned]
+    pool.free(ints([0, 1, 2]))
+    model.free([0, 1, 2])
+    before = model.refs.copy()
+    moved = torch.full((40,), -9, dtype=torch.int32, device="cuda")
+    assert pool.compact(moved).tolist() == [model.compact()] == [12]
+    model.same(pool, keys, values)
+    to = moved.tolist()
+    live = [p for p in range(40) if before[p] > 0]
+    assert sorted(to[p] for p in live) == list(range(12)) and all(to[p] == p for p in range(40) if before[p] <= 0 or p < 12)
+    assert [to[p] for p in live if p >= 12] == [p for p in range(12) if before[p] <= 0]
+    assert pool.extend(ints([5]), ints([70])).tolist() == model.extend([5], [70]) == [OK]
+    model.same(pool, keys, values)
+    for p, want in zip(pinned, held):
+        assert all(torch.equal(t[to[p]].view(torch.int16), w.view(torch.int16)) for t, w in zip((*keys, *values), want))
+        assert to[p] not in pool.page_tables[5].tolist()
+        pool.refcounts[to[p]] -= 1
+        model.refs[to[p]] -= 1
+    # nothing moves now that pages 0 .. live - 1 are live but for those that were given back; a pool without holes says so
+    pool.free(ints([3]))
+    model.free([3])
+    assert pool.compact(moved).tolist() == [model.compact()]
+    model.same(pool, keys, values)
+    assert pool.compact(moved).tolist() == [model.compact()] and moved.tolist() == list(range(40))
+    for bad in (moved[:39], moved.long(), moved.cpu()):
+        with pytest.raises(ValueError):
+            pool.compact(bad)
+
+
 def test_refusals():
     pool, keys, values, _ = make(1, 8, 4, 1, 8, 4, 4)
     for bad in (lambda: pool.extend(ints([0, 1]), ints([1])), lambda: pool.extend(torch.zeros(1, dtype=torch.int64, device="cuda"), ints([1])),
