@@ -1,4 +1,4 @@
-// What the chunk attention kernels share: the operands of one call, the addressing of the paged cache, and the row loop.
+// What the chunk attention kernels share: the operands of one call and the addressing of the paged cache.
 #pragma once
 #include "common.cuh"
 
@@ -67,40 +67,6 @@ __device__ __forceinline__ long long chunk_cache_offset(const Chunk& p, int b, i
     if (page < 0 || page >= p.physical_pages) return -1;
     return (((long long)page * p.page_size + slot % p.page_size) * p.kv_heads + head) * kChDim;
 }
-
-__device__ __forceinline__ float chunk_warp_sum(float v)
-{
-#pragma unroll
-    for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
-    return v;
-}
-
-// One (row, q head) by one warp, slot after slot: running maximum and sum in fp32, four dims per lane.
-__device__ __forceinline__ void chunk_row(const Chunk& p, int b, int row, int head, int slot, int lane)
-{
-    const int group = p.q_heads / p.kv_heads, kv = head / group;
-    const uint2 qr = *(reinterpret_cast<const uint2*>(p.queries + ((size_t(kv) * p.tokens + row) * group + head % group) * kChDim) + lane);
-    const float q[4] = {__uint_as_float(qr.x << 16), __uint_as_float(qr.x & 0xffff0000u), __uint_as_float(qr.y << 16), __uint_as_float(qr.y & 0xffff0000u)};
-    float top = -INFINITY, sum = 0.f, o[4] = {};
-    for (int s = 0; s <= slot; ++s) {
-        const long long at = chunk_cache_offset(p, b, s, kv);
-        if (at < 0) continue;
-        const uint2 kr = *(reinterpret_cast<const uint2*>(p.keys + at) + lane), vr = *(reinterpret_cast<const uint2*>(p.values + at) + lane);
-        const float score = chunk_warp_sum(q[0] * __uint_as_float(kr.x << 16) + q[1] * __uint_as_float(kr.x & 0xffff0000u) +
-                                           q[2] * __uint_as_float(kr.y << 16) + q[3] * __uint_as_float(kr.y & 0xffff0000u)) * 0.08838834764831845f;
-        if (score == -INFINITY) continue;   // weight 0
-        const float next = fmaxf(top, score), old = top == next ? 1.f : expf(top - next), w = expf(score - next);
-        const float v[4] = {__uint_as_float(vr.x << 16), __uint_as_float(vr.x & 0xffff0000u), __uint_as_float(vr.y << 16), __uint_as_float(vr.y & 0xffff0000u)};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = o[i] * old + w * v[i];
-        sum = sum * old + w;
-        top = next;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const __nv_bfloat162 r[2] = {__floats2bfloat162_rn(o[0] * inv, o[1] * inv), __floats2bfloat162_rn(o[2] * inv, o[3] * inv)};
-    *(reinterpret_cast<uint2*>(p.out + (size_t(row) * p.q_heads + head) * kChDim) + lane) = *reinterpret_cast<const uint2*>(r);
-}
-
 #endif
 
 struct ChunkPlan;

@@ -25,10 +25,10 @@
 // for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
 // Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  The tensor core cuts towards zero what it adds to a
 // sum: O is taken out of tensor memory every kChSumSteps steps and added in fp32, in memory of the workspace (19 MB, which stay in L2)
-// of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its rounding and what that left out: 16 of its
-// bits, 2^-16 of it at most lost, where one number (half as many MMAs of P V: 315 instead of 383 us a call of 8192 rows before sums
-// were kept apart) loses 2^-8, about what the result's own rounding takes.  A row that comes out NaN (infinities in places that it does
-// not see meet weights of zero) is computed again by the row loop.
+// of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its first bits and the rest: 2^-15 of it is lost
+// at most, where one number (half as many MMAs of P V: 315 instead of 383 us a call of 8192 rows before sums were kept apart) loses
+// 2^-8, about what the result's own rounding takes.  A row that comes out NaN though its scores are numbers, and that does not see one of
+// the block's values that is not finite (its weight of zero makes NaN of it), is computed again by the row loop.
 #include <algorithm>
 #include <cooperative_groups.h>
 
@@ -52,7 +52,16 @@ __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("ba
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 constexpr int kKeys = 64;         // keys of a step (UMMA N of Q K^T, K of P V)
 constexpr int kChRounds = kKeys / 32;   // P is handed over, and rows are copied, 32 keys at a time
-constexpr int kPieces = 2;        // bf16 numbers that a weight of P enters P V as
+// A weight of P enters P V as two bf16 numbers, cut off and rest: both of them positive, the rest by 2^-20 of the weight where nothing is
+// left, so that an infinite value stays infinite (of two numbers of opposite signs, or a zero, it would make NaN).
+constexpr int kPieces = 2;
+constexpr float kNearlyOne = 1.f - 0x1p-20f;
+__device__ __forceinline__ uint32_t bf16x2_cut(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
 constexpr int kChExists = 16;     // steps whose key bits are kept
 
 template <int kTiles, int kUnits>
@@ -76,6 +85,87 @@ struct ChShape {
     static constexpr uint32_t col_o = 2 * kKeys, tile_cols = col_o + kChDim, cols = kTiles * tile_cols;
     static_assert(kTiles * tile_cols <= 512, "tensor memory");
 };
+
+__device__ __forceinline__ float chunk_warp_sum(float v)
+{
+#pragma unroll
+    for (int off = 16; off; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+    return v;
+}
+
+// One (row, q head) by one warp, eight slots at a time: running maximum and sum in fp32, four dims per lane.  A score of NaN or +inf makes
+// the row NaN; one of -inf has weight 0, whatever the value there.
+__device__ __noinline__ void chunk_row(const Chunk& p, int b, int row, int head, int slot, int lane)
+{
+    constexpr int kAtOnce = 8;
+    const int group = p.q_heads / p.kv_heads, kv = head / group;
+    const uint2 qr = *(reinterpret_cast<const uint2*>(p.queries + ((size_t(kv) * p.tokens + row) * group + head % group) * kChDim) + lane);
+    const float q[4] = {__uint_as_float(qr.x << 16), __uint_as_float(qr.x & 0xffff0000u), __uint_as_float(qr.y << 16), __uint_as_float(qr.y & 0xffff0000u)};
+    float top = -INFINITY, sum = 0.f, o[4] = {};
+    for (int s0 = 0; s0 <= slot; s0 += kAtOnce) {
+        uint2 kr[kAtOnce], vr[kAtOnce];
+        uint32_t there = 0;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const long long at = s0 + i <= slot ? chunk_cache_offset(p, b, s0 + i, kv) : -1;
+            kr[i] = vr[i] = make_uint2(0, 0);
+            if (at < 0) continue;
+            there |= 1u << i;
+            kr[i] = *(reinterpret_cast<const uint2*>(p.keys + at) + lane), vr[i] = *(reinterpret_cast<const uint2*>(p.values + at) + lane);
+        }
+        float score[kAtOnce], next = top;
+        bool wild = false;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            score[i] = chunk_warp_sum(q[0] * __uint_as_float(kr[i].x << 16) + q[1] * __uint_as_float(kr[i].x & 0xffff0000u) +
+                                      q[2] * __uint_as_float(kr[i].y << 16) + q[3] * __uint_as_float(kr[i].y & 0xffff0000u)) * 0.08838834764831845f;
+            if (!((there >> i) & 1)) score[i] = -INFINITY;
+            wild = wild || !(score[i] < INFINITY);
+            next = fmaxf(next, score[i]);
+        }
+        if (wild) {   // the same for all lanes
+            sum = NAN;
+            break;
+        }
+        if (next == -INFINITY) continue;
+        const float old = top == next ? 1.f : expf(top - next);
+        sum *= old;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[d] *= old;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            if (score[i] == -INFINITY) continue;   // weight 0
+            const float w = expf(score[i] - next);
+            const float v[4] = {__uint_as_float(vr[i].x << 16), __uint_as_float(vr[i].x & 0xffff0000u), __uint_as_float(vr[i].y << 16), __uint_as_float(vr[i].y & 0xffff0000u)};
+#pragma unroll
+            for (int d = 0; d < 4; ++d) o[d] += w * v[d];
+            sum += w;
+        }
+        top = next;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const __nv_bfloat162 r[2] = {__floats2bfloat162_rn(o[0] * inv, o[1] * inv), __floats2bfloat162_rn(o[2] * inv, o[3] * inv)};
+    *(reinterpret_cast<uint2*>(p.out + (size_t(row) * p.q_heads + head) * kChDim) + lane) = *reinterpret_cast<const uint2*>(r);
+}
+
+// The last of the slots [from, to) of sequence b at which a head's value is not finite, -1 without one; by one warp, eight at a time.
+__device__ __noinline__ int chunk_last_wild(const Chunk& p, int b, int kv, int from, int to, int lane)
+{
+    constexpr int kAtOnce = 8;
+    const auto wild = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+    for (int s0 = to - 1; s0 >= from; s0 -= kAtOnce) {
+        uint2 v[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const long long at = s0 - i >= from ? chunk_cache_offset(p, b, s0 - i, kv) : -1;
+            v[i] = at >= 0 ? *(reinterpret_cast<const uint2*>(p.values + at) + lane) : make_uint2(0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i)
+            if (__any_sync(0xffffffffu, wild(v[i].x) || wild(v[i].y))) return s0 - i;
+    }
+    return -1;
+}
 
 // A warp takes a slot, the first free one from `from` on: there are as many as there can be tiles that hold tensor memory, as this one
 // does.  (One that all want first takes the last of 256 tiles 15 us; looking at one after the other, 1 us each.)
@@ -128,7 +218,7 @@ __device__ __forceinline__ bool wait_warp(uint64_t* bar, uint32_t parity, volati
 
 template <int kTiles, int kUnits>
 __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 ? 2 : 1)
-    attn_chunk_tc_kernel(const Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
+    attn_chunk_tc_kernel(const __grid_constant__ Chunk p, const __grid_constant__ CUtensorMap q_map, const int splits)
 {
     using S = ChShape<kTiles, kUnits>;
     extern __shared__ uint8_t smem_raw[];
@@ -459,7 +549,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                 }
             }
             const float base = ref == -INFINITY ? 0.f : ref;
-            const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base), minus1 = f32x2(-1.f, -1.f);
+            const uint64_t scale2 = f32x2(kScale, kScale), base2 = f32x2(-base, -base), minus1 = f32x2(-kNearlyOne, -kNearlyOne);
             uint64_t part2[2] = {0, 0};
             if (j < turns && (q == 1 || j > 0)) bar_sync(kBarTurn + q, 256);
 #pragma unroll
@@ -472,7 +562,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                     const uint64_t both = f32x2(ex2(a), ex2(d));
                     part2[i & 1] = add2(part2[i & 1], both);
                     f32x2_split(both, a, d);
-                    w[i] = bf16x2_of(a, d);
+                    w[i] = bf16x2_cut(a, d);
                     f32x2_split(fma2(f32x2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), minus1, both), a, d);
                     rest[i] = bf16x2_of(a, d);
                 }
@@ -530,7 +620,14 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                 }
             }
             __syncwarp();
-            for (uint32_t redo = __ballot_sync(0xffffffffu, bad && good); redo; redo &= redo - 1) {
+            // a sum of weights that is NaN says so rightly; another, only where no value that the row does not see is to blame
+            bad = bad && good && !isnan(sum);
+            uint32_t redo = __ballot_sync(0xffffffffu, bad);
+            if (redo) {
+                const int wild = chunk_last_wild(p, blk.b, kv, __reduce_min_sync(0xffffffffu, bad ? end : most), most, lane);
+                redo = __ballot_sync(0xffffffffu, bad && (end <= wild || sum == 0.f));
+            }
+            for (; redo; redo &= redo - 1) {
                 const int from = __ffs(redo) - 1;
                 chunk_row(p, blk.b, __shfl_sync(0xffffffffu, blk.row0 + t, from), __shfl_sync(0xffffffffu, head, from), __shfl_sync(0xffffffffu, end, from) - 1, lane);
             }
@@ -600,8 +697,13 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
                 }
             }
             __syncwarp();
-            const uint32_t redo = __ballot_sync(0xffffffffu, bad);
-            if (redo && !*abort_flag)
+            bad = bad && !*abort_flag && !isnan(total);
+            uint32_t redo = __ballot_sync(0xffffffffu, bad);
+            if (redo) {   // as above
+                const int wild = chunk_last_wild(p, blk.b, kv, __reduce_min_sync(0xffffffffu, bad ? end : most), most, lane);
+                redo = __ballot_sync(0xffffffffu, bad && end <= wild);
+            }
+            if (redo)
                 for (int g = 0; g < 4; ++g)
                     if ((redo >> (8 * g)) & 0xffu)
                         chunk_row(p, blk.b, __shfl_sync(0xffffffffu, row, 8 * g), __shfl_sync(0xffffffffu, head, 8 * g), __shfl_sync(0xffffffffu, end, 8 * g) - 1, lane);

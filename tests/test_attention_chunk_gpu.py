@@ -452,3 +452,61 @@ def test_the_decode_kernel_and_pages_that_do_not_exist():
     assert all((g[0] == 3).all() and (g[-1] == 3).all() for g in guard)
     assert np.array_equal(guard[1][1:-1].float().cpu().numpy(), values)
     assert (np.abs(guard[0][1:-1].float().cpu().numpy() - keys) <= 2.0 ** -7 * np.abs(keys)).all()      # k by plain fp32 steps: a neighbour at most
+
+
+@pytest.mark.parametrize("what", ["a key of the context", "a key of the chunk", "a query", "a value of the context"])
+@pytest.mark.parametrize("tokens", [512, 3])
+def test_rows_that_are_nan_cost_no_more_than_others(what, tokens):
+    """A NaN that most rows of one sequence see: those of its kv head are NaN, all others have the bits that they have without it, and the
+    call takes no longer than a few others (walked through one slot after the other, 512 such rows at 30000 took 100 times as long)."""
+    cfg, start = dec.DecoderConfig(q_heads=16, kv_heads=8), 30000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    pages = (start + tokens) // 16 + 1
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    keys, values = (torch.randn(2 * pages, 16, 8, 128, device="cuda", generator=gen).to(torch.bfloat16) for _ in range(2))
+    qkv = torch.randn(2 * tokens, 32, 128, device="cuda", generator=gen).to(torch.bfloat16)
+    one = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(16 * pages, 128, cfg.rope_theta))
+    op = dec.ChunkAttention(cfg, 2 * tokens, 16 * pages, pages, 16 * pages)
+    table = torch.randperm(2 * pages, device="cuda", generator=gen).to(torch.int32).view(2, pages)
+
+    def run():
+        out = torch.zeros(2 * tokens, 16 * 128, dtype=torch.bfloat16, device="cuda")
+        begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        begin.record()
+        op.run(qkv.view(2 * tokens, -1), one, one, cos, sin, keys, values, table, ints(start, start), ints(0, tokens, 2 * tokens), out)
+        end.record()
+        torch.cuda.synchronize()
+        return out.view(2, tokens, 16, 128), begin.elapsed_time(end)
+
+    run()
+    clean, _ = run()
+    first = 0                                            # row of sequence 0 from which on results are NaN
+    hit = torch.zeros(16, 128, dtype=torch.bool, device="cuda")
+    hit[6:8] = True
+    if what == "a key of the context":
+        keys[table[0, 0], 5, 3, 17] = float("nan")
+    elif what == "a key of the chunk":
+        qkv[0, 16 + 3, 17] = float("nan")
+    elif what == "a query":
+        qkv[:tokens, 6:8, 17] = float("nan")
+    else:
+        values[table[0, 0], 5, 3, 17] = float("nan")
+        hit[:] = False
+        hit[6:8, 17] = True
+    got, ms = run()
+    assert got[0, first:, hit].isnan().all()
+    assert torch.equal(got[0][:, ~hit], clean[0][:, ~hit]) and torch.equal(got[1], clean[1])
+    assert ms < 5, f"{ms} ms"
+
+
+def test_values_that_rows_do_not_see_and_values_that_they_see():
+    """Infinities and NaN in both: rows before the last of them are what they are without it, dims with one that a row sees are NaN."""
+    for lens, starts, heads in (([150], [700], (2, 1)), ([9], [3000], (4, 1)), ([150, 20], [40, 90], (16, 8))):
+        c = Case(lens, starts, *heads, seed=31)
+        h, kv = heads
+        x = c.qkv.view(-1, h + 2 * kv, 128)
+        for row, dim, value in ((lens[0] // 2, 3, float("inf")), (lens[0] - 1, 4, float("nan")), (lens[0] // 3, 5, -float("inf"))):
+            x[row, h + kv, dim] = value
+        c.values[c.table[0, 1], 2, 0, 6] = float("nan")
+        c.check()

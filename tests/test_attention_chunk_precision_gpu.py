@@ -1,11 +1,11 @@
 """How exact chunk attention is beside its results' own rounding: weights of 16 bits, sums that do not lose with the length of the context.
 
 Tolerances, relative to the value or to mass = sum p |v|.  A result's rounding to bf16 is half a step, 2^-8 at most.  A weight enters its
-product with v as two bf16 numbers: 2^-8 of 2^-8 of it is left out, 2^-16.  The scores of these cases stay below 2^4 in powers of two and
-their 128 products below 2^7: the tensor core cuts them eight times at 2^-17 each, 2^-14 in the sum and 2^-17 in the exponent after the
-scale 1 / sqrt(128) log2 e = 2^-3; the exponent's own rounding and the exponential add 2^-19.  Sums of up to 600 positions lose 2^-23 of
-themselves per MMA of eight per 64 positions at most, half of that on average over their growth: 2^-18.  In all less than 2^-15 of the mass,
-twice (result and denominator): 2^-14."""
+product with v as two bf16 numbers, eight bits cut off and eight rounded: 2^-7 2^-8 = 2^-15 of it is left out at most.  The scores of
+these cases stay below 2^4 in powers of two and their 128 products below 2^7: the tensor core cuts them eight times at 2^-17 each, 2^-14 in
+the sum and 2^-17 in the exponent after the scale 1 / sqrt(128) log2 e = 2^-3; the exponent's own rounding and the exponential add 2^-19,
+both in the result and in its denominator.  Sums of up to 600 positions lose 2^-23 of themselves per MMA of eight per 64 positions at most,
+half of that on average over their growth: 2^-18.  In all 2^-15 (1 + 2 (1/4 + 1/16) + 1/8), less than 2^-14 of the mass."""
 import numpy as np
 import pytest
 import torch
