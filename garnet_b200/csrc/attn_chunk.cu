@@ -140,7 +140,8 @@ __global__ void __launch_bounds__(kRowThreads, 8) attn_chunk_rows_kernel(const C
     }
     if (__any_sync(0xffffffffu, turns)) {
         // packed: dims 8 l + 2 i, 8 l + 2 i + 1, and from i = 4 on those 64 further on
-        const uint32_t xs[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w}, ws[8] = {wlo.x, wlo.y, wlo.z, wlo.w, whi.x, whi.y, whi.z, whi.w};
+        const uint32_t xs[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        uint32_t ws[8] = {wlo.x, wlo.y, wlo.z, wlo.w, whi.x, whi.y, whi.z, whi.w};
         const uint64_t minus1 = f32x2(-1.f, -1.f);
         uint64_t sum2 = 0, rest2 = 0;   // the sum of squares and what it is short of
 #pragma unroll
@@ -166,9 +167,15 @@ __global__ void __launch_bounds__(kRowThreads, 8) attn_chunk_rows_kernel(const C
         }
         const float high = sum * (1.f / kChDim), low = __fmaf_rn(rest, 1.f / kChDim, p.eps), mean = __fadd_rn(high, low);
         const float short_of = __fsub_rn(low, __fsub_rn(mean, high));
-        const float r = 1.f / sqrtf(mean), square = __fmul_rn(mean, r);
+        float r = 1.f / sqrtf(mean);
+        const float square = __fmul_rn(mean, r);
         // what r is short of 1 / sqrt(mean)
-        const float c = 0.5f * r * (__fmaf_rn(-square, r, 1.f) - __fmaf_rn(mean, r, -square) * r - short_of * r * r);
+        float c = 0.5f * r * (__fmaf_rn(-square, r, 1.f) - __fmaf_rn(mean, r, -square) * r - short_of * r * r);
+        if (sum == INFINITY) {   // squares beyond fp32: numbers become 0, infinities NaN
+            r = c = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ws[i] = 0x3f803f80u;   // one: a product with the weight could be infinite
+        }
         if (turns) {
             const uint64_t r2 = f32x2(r, r), c2 = f32x2(c, c);
             uint64_t n[8];

@@ -85,3 +85,29 @@ def test_maxima_that_grow_along_a_long_context(lens, starts, heads):
     off = np.abs(d["out"].double().cpu().numpy() - want)
     bad = off > 2.0 ** -8 * np.abs(want) + 2.0 ** -13 * mass
     assert not bad.any(), f"{bad.sum()} of {bad.size}"
+
+
+def test_squares_beyond_fp32():
+    """Heads whose squares overflow come out as zeros, as the one-token kernel has them; an infinity among them is NaN."""
+    cfg = dec.DecoderConfig(q_heads=4, kv_heads=2)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(64, 128, cfg.rope_theta))
+    w = torch.full((128,), 3.0, dtype=torch.bfloat16, device="cuda")
+    qkv = torch.randn(3, 8, 128, device="cuda", generator=gen)
+    qkv[0, 4] *= 2.0 ** 66                       # a key
+    qkv[1, 0] *= 2.0 ** 126                      # a query: its product with the weight overflows too
+    qkv[1, 4, 7] = 2.0 ** 65                     # one value of a key
+    qkv[2, 5, 9] = float("inf")
+    qkv = qkv.to(torch.bfloat16)
+    got, want = [], []
+    for results, op, more in ((got, dec.ChunkAttention(cfg, 3, 64, 4, 64), (ints(0, 1, 2, 3),)), (want, dec.PagedAttention(cfg, 3, 64, 4, 64), ())):
+        keys, values = (torch.zeros(12, 16, 2, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        out = torch.zeros(3, 4 * 128, dtype=torch.bfloat16, device="cuda")
+        op.run(qkv.view(3, -1), w, w, cos, sin, keys, values, torch.arange(12, dtype=torch.int32, device="cuda").view(3, 4), ints(5, 0, 20), *more, out)
+        results += [out.view(3, 4, 128), keys]
+    assert (got[1][0, 5, 0] == 0).all() and (got[1][4, 0, 0] == 0).all() and got[1][9, 4, 1].isnan().any()
+    assert torch.equal(got[1].isnan(), want[1].isnan()) and torch.equal(got[1][4, 0, 0], want[1][4, 0, 0])
+    assert torch.equal(got[0][:2], want[0][:2])          # one slot each: the value itself
+    # a score of NaN: softmax is NaN (the one-token kernel leaves out what has such a sum)
+    assert got[0][2, 2:].isnan().all() and not got[0][2, :2].isnan().any()
