@@ -31,8 +31,8 @@ __device__ __forceinline__ uint32_t narrow(uint64_t v)
 
 // A warp takes four heads of a row, eight lanes each: dims 8 l .. 8 l + 7 and the eight 64 further on, which RoPE turns together.
 // Rounded to bf16 after the norm and after the rotation, as a bf16 network does; the fp32 steps in between carry what the sum of
-// squares, the products and the root are short of: some 1 of 10^6 results is the other bf16 neighbour of the float64 result (10 to
-// 20 of 10^6 by plain fp32 steps).
+// squares, the products and the root are short of: of 10^6 keys of normal rows 1.7 differ from the float64 result rounded to fp32 and then to
+// bf16 (25 by plain fp32 steps).
 // Bound: HBM in principle, the rows in and q, k and v out; in practice its instructions, some 250 for four heads with two values to an
 // instruction.
 constexpr int kRowThreads = 128;

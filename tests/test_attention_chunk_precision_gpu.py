@@ -87,6 +87,38 @@ def test_maxima_that_grow_along_a_long_context(lens, starts, heads):
     assert not bad.any(), f"{bad.sum()} of {bad.size}"
 
 
+def test_keys_of_general_rows_are_the_rounded_float64_results():
+    """Norm and RoPE of normal rows against float64, rounded to fp32 and then to bf16.  The kernel carries what its fp32 steps are short of: its
+    fp32 number before the norm's rounding to bf16 is the rounded float64 one; before RoPE's it has been rounded twice, so that it is a
+    neighbour in half of the cases at most, and one gap of fp32 numbers in 2^16 changes the bf16 number: 2^-17, 8 of 10^6 (plain fp32 steps
+    have 25)."""
+    cfg, tokens = dec.DecoderConfig(q_heads=8, kv_heads=8), 4096
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(tokens, 128, cfg.rope_theta))
+    w = (1 + 0.2 * torch.randn(128, device="cuda", generator=gen)).to(torch.bfloat16)
+    one = torch.ones(128, dtype=torch.bfloat16, device="cuda")
+    op = dec.ChunkAttention(cfg, tokens, tokens, tokens // 16, tokens)
+    off = plain = count = 0
+    for _ in range(4):
+        qkv = torch.randn(tokens, 24, 128, device="cuda", generator=gen).to(torch.bfloat16)
+        keys, values = (torch.zeros(tokens // 16, 16, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        out = torch.empty(tokens, 8 * 128, dtype=torch.bfloat16, device="cuda")
+        op.run(qkv.view(tokens, -1), one, w, cos, sin, keys, values, torch.arange(tokens // 16, dtype=torch.int32, device="cuda")[None], ints(0), ints(0, tokens), out)
+        x = qkv[:, 8:16].double()
+        x = (x * (x.pow(2).mean(-1, keepdim=True) + float(np.float32(cfg.eps))).rsqrt() * w.double()).float().to(torch.bfloat16).double()
+        a, b, c, s = x[..., :64], x[..., 64:], cos.double()[:, None], sin.double()[:, None]
+        want = torch.cat([a * c - b * s, b * c + a * s], -1).float().to(torch.bfloat16)
+        off += int((keys.view(tokens, 8, 128) != want).sum())
+        y = qkv[:, 8:16].float()
+        y = (y / torch.sqrt((y * y).mean(-1, keepdim=True) + cfg.eps) * w.float()).to(torch.bfloat16).float()
+        a, b, c, s = y[..., :64], y[..., 64:], cos[:, None], sin[:, None]
+        plain += int((torch.cat([a * c - b * s, b * c + a * s], -1).to(torch.bfloat16) != want).sum())
+        count += want.numel()
+    print(f"{off / count * 1e6:.1f} of 10^6, plain fp32 steps {plain / count * 1e6:.1f}")
+    assert off <= 8e-6 * count, f"{off} of {count}"
+
+
 def test_squares_beyond_fp32():
     """Heads whose squares overflow come out as zeros, as the one-token kernel has them; an infinity among them is NaN."""
     cfg = dec.DecoderConfig(q_heads=4, kv_heads=2)
