@@ -62,12 +62,14 @@ inline int oss_prefill_tiles(int batch, int kv_heads, int tokens, int tile_token
 // Chunk attention (attn_chunk_tc.cu): tiles of 128 query rows per CTA, steps of keys that its ring holds (`units`), and CTAs of a
 // cluster that share a tile's keys.  Three kinds of CTA: two tiles on the same keys, for long work; one tile with a ring of six
 // steps, which hides the reads' latency where an SM has one CTA; one tile with a ring of two, of which two CTAs fit an SM.  The kind
-// and the shares with the least estimated time are taken, the time being waves x (fixed part + steps x step), with figures
-// measured on a B200: a step of 64 keys takes 0.95, 0.74 and 0.9 us (1.3 us when two CTAs share the SM), the fixed part is 8, 6 and
-// 5 us, shares add 3 us.  Over 23 shapes from 1 to 8192 tokens at 0 to 30000 earlier ones, against the best of 12 plans each, it
-// takes 1.01 times as long on average and 1.12 at worst (24 equal sequences of one token at 3500: 88 us, 79 in four shares).
-// The plainer rule of two tiles where every SM then has a CTA, and otherwise one tile and shares for twice the SMs, took 162 instead
-// of 138 us for 512 tokens at 30000, and 34 instead of 24 us for 4 x 5 tokens at 4000.
+// and the shares with the least estimated time are taken, the time being waves x (fixed part + steps x step), with figures fitted to
+// what a B200 takes: a fixed part of 7, 6 and 5 us, a step of 64 keys of 1.1, 0.74 and 1.3 us (0.95, 0.82 and 1.0 us where every CTA has
+// an SM to itself), 5 us for shares.  Over 25 shapes from 1 to 8192 tokens at 0 to 30000 earlier ones it takes 1.02 times as long as the
+// best of the 12 plans on average and 1.17 at worst (64 ragged sequences of up to 4 tokens at up to 4000: 89 us, 76 in two shares).
+// `max_context` is the call's: with 32768 in its place the short calls of these shapes are cut up too far.  A prompt of 128 tokens then takes
+// 19 instead of 10 us, 512 tokens 22 instead of 17, 2048 tokens 52 instead of 46, 256 tokens at 3000 45 instead of 25, 24 x 5 tokens at up
+// to 3500 66 instead of 52, 8 ragged prompts 93 instead of 64, 32 x up to 200 tokens at up to 900 107 instead of 71, 8 x up to 512 at up to
+// 2000 92 instead of 68; the other 17 within 13 %.
 struct ChunkPlan {
     int tiles, units, splits;
 };
@@ -77,7 +79,7 @@ inline ChunkPlan chunk_plan(int batch, int kv_heads, int tokens, int tile_tokens
         int tiles, units, per_sm;
         double fixed, step, alone;
     };
-    constexpr Kind kinds[3] = {{1, 2, 2, 5.0, 1.3, 0.9}, {2, 5, 1, 8.0, 0.95, 0.95}, {1, 6, 1, 6.0, 0.74, 0.74}};
+    constexpr Kind kinds[3] = {{1, 2, 2, 5.0, 1.3, 1.0}, {2, 5, 1, 7.0, 1.1, 0.95}, {1, 6, 1, 6.0, 0.74, 0.82}};
     const long long each = (tokens + batch - 1) / batch;   // rows of a sequence, were they all as long
     ChunkPlan best = {1, 2, 1};
     double least = -1.0;
@@ -90,7 +92,7 @@ inline ChunkPlan chunk_plan(int batch, int kv_heads, int tokens, int tile_tokens
             const long long steps = ((keys + 63) / 64 + splits - 1) / splits;
             double waves = std::max(1.0, double(ctas) / double(room));
             if (waves < 2.0 && waves > 1.0) waves = 0.6 * waves + 0.8;   // a second wave that is not full still takes most of a wave
-            const double time = waves * (k.fixed + double(steps) * (ctas <= kSmCount ? k.alone : k.step) + (splits > 1 ? 3.0 : 0.0));
+            const double time = waves * (k.fixed + double(steps) * (ctas <= kSmCount ? k.alone : k.step) + (splits > 1 ? 5.0 : 0.0));
             if (least < 0.0 || time < least) least = time, best = {k.tiles, k.units, splits};
         }
     }

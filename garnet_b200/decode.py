@@ -90,7 +90,11 @@ class ChunkAttention:
     """garnet_b200_attention_chunk with its workspace: attention of a chunk of new tokens of each of several sequences - a prompt, a
     further piece of one, drafted tokens to verify - which PagedAttention does for one token each.  `run` takes up to `max_tokens` rows
     of `qkv` [rows, (q_heads + 2 kv_heads) * 128] bf16; sequence b has the rows row_starts[b] .. row_starts[b + 1] - 1 (int32 [batch + 1])
-    at the slots positions[b], positions[b] + 1, ... of page_tables[b].  The object's workspace serves one call at a time."""
+    at the slots positions[b], positions[b] + 1, ... of page_tables[b].  The object's workspace serves one call at a time.
+
+    `context` of a call: the most slots that a row of it sees, where the host knows it (rows behind them come out as zeros, as those behind
+    max_context do).  The call is cut into CTAs by it: a prompt of 2048 rows takes longer on an object for 32768 slots than on one for 2048
+    unless it is told (figures in launch_plan.h)."""
 
     def __init__(self, cfg: DecoderConfig, max_tokens: int, max_context: int, max_logical_pages: int, rope_positions: int):
         self.opt = AttentionOptions(abi=1, struct_size=ctypes.sizeof(AttentionOptions), q_heads=cfg.q_heads, kv_heads=cfg.kv_heads,
@@ -104,7 +108,8 @@ class ChunkAttention:
         self._dims = (cfg.qkv_width, (cfg.head_dim,), cfg.head_dim // 2, rope_positions, (cfg.page_size, cfg.kv_heads, cfg.head_dim),
                       max_logical_pages, cfg.q_heads * cfg.head_dim)
 
-    def run(self, qkv, q_norm_w, k_norm_w, cos, sin, key_pages, value_pages, page_tables, positions, row_starts, out, pdl: bool = False):
+    def run(self, qkv, q_norm_w, k_norm_w, cos, sin, key_pages, value_pages, page_tables, positions, row_starts, out, pdl: bool = False,
+            context: Optional[int] = None):
         bf, f32, i32, d = torch.bfloat16, torch.float32, torch.int32, self._dims
         rows, batch, pages, angles = qkv.shape[0], positions.numel(), key_pages.shape[0], cos.shape[0]
         tensors = ((qkv, bf, (rows, d[0])), (q_norm_w, bf, d[1]), (k_norm_w, bf, d[1]), (cos, f32, (angles, d[2])), (sin, f32, (sin.shape[0], d[2])),
@@ -118,8 +123,15 @@ class ChunkAttention:
             raise ValueError(f"cos and sin must have {d[3]} rows or more")
         if self.ws.get_device() != qkv.get_device():
             raise ValueError("the workspace is on another device than the rows")
+        opt = self._opt
+        if context is not None:
+            if not 1 <= context <= self.opt.max_context:
+                raise ValueError(f"context must lie between 1 and max_context, {self.opt.max_context}")
+            own = AttentionOptions.from_buffer_copy(self.opt)
+            own.max_context = context
+            opt = ctypes.byref(own)
         if batch and rows:
-            check(self._call(self._opt, qkv.data_ptr(), q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+            check(self._call(opt, qkv.data_ptr(), q_norm_w.data_ptr(), k_norm_w.data_ptr(), cos.data_ptr(), sin.data_ptr(),
                              key_pages.data_ptr(), value_pages.data_ptr(), page_tables.data_ptr(), positions.data_ptr(),
                              row_starts.data_ptr(), out.data_ptr(), self._ws, self._ws_bytes, batch, rows, pages, 1 if pdl else 0, stream_ptr()))
         return out

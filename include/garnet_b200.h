@@ -333,12 +333,15 @@ int garnet_b200_attention_decode(const garnet_b200_attention_options* options, c
  * slots behind it.  Every row is treated as by garnet_b200_attention_decode - head norms, RoPE, k and v appended to the cache - and
  * sees the slots up to its own, those that the call itself appends included.  `tokens` is the number of rows of d_qkv
  * [tokens, (q_heads + 2 kv_heads) * 128] and d_out [tokens, q_heads * 128] (bf16); rows of no sequence are left as they are.
- *   - A row whose slot is negative, or not below max_context, appends nothing and comes out as zeros.
+ *   - All rows of a sequence whose first slot is negative, and rows whose slot is not below max_context, append nothing and come out as
+ *     zeros.
  *   - Slots whose page is not one of the `physical_pages` of the cache are not written and not seen; a row that sees none is zeros.
  *   - What the cache holds behind a sequence's last slot does not matter (NaN and infinities included).
  *   - Pages that hold the slots of new rows belong to one sequence each; full pages before them may be shared.
  *   - q_heads / kv_heads at most 128.  Rows, cache pages, norm weights, rope tables and output start on 16-byte boundaries.
- * Weights enter their products with the values with 16 bits, all sums are fp32.
+ * Weights enter their products with the values with 16 bits (2^-15 of a weight is lost at most), all sums are fp32.
+ * The call is cut into CTAs by max_context.  Where the host knows how far the rows of a call reach, it gives the call options with that
+ * number; the workspace for the larger one serves.
  * The workspace (garnet_b200_attention_chunk_workspace for that many rows, 256-byte aligned; 19 MB of it for sums where max_context is
  * above 4096) needs no clearing and holds nothing between calls; calls that overlap on the GPU need one each.  flags bit 0:
  * programmatic dependent launch.  No allocation, no synchronisation.  The reference runs prompts through the same engines, cache append and page tables as its decode step

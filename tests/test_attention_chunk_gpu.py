@@ -510,3 +510,36 @@ def test_values_that_rows_do_not_see_and_values_that_they_see():
             x[row, h + kv, dim] = value
         c.values[c.table[0, 1], 2, 0, 6] = float("nan")
         c.check()
+
+
+@pytest.mark.parametrize("lens,starts,heads", [([130], [0], (16, 8)), ([5, 2, 0], [700, 1000, 3], (4, 2))])
+def test_a_call_that_says_how_far_its_rows_reach(lens, starts, heads):
+    """An object for 40000 slots: told the call's context it gives the bits of an object for just that; rows behind what it is told are zeros and
+    append nothing."""
+    c = Case(lens, starts, *heads, seed=41)
+    want = c.run()
+    reach, width, room = max(n + s for n, s in zip(lens, starts)), 2500, 40000
+    fitted = dec.ChunkAttention(c.cfg, c.rows, reach, c.width, c.positions_room)
+    cos, sin = (torch.from_numpy(t).cuda() for t in dec.rope_tables(room, 128, c.cfg.rope_theta))
+    large = dec.ChunkAttention(c.cfg, c.rows + 3, room, width, room)
+    table = torch.full((c.batch, width), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.width] = c.table.cuda()
+    results = []
+    for op, more in ((fitted, {}), (large, dict(cos=cos, sin=sin, page_tables=table, context=reach)), (large, dict(cos=cos, sin=sin, page_tables=table)),
+                     (large, dict(cos=cos, sin=sin, page_tables=table, context=reach - 1))):
+        d = c.device()
+        op.run(**dict(d, **more))
+        results.append(d)
+    a, b, far, less = results
+    for name in ("out", "key_pages", "value_pages"):
+        assert torch.equal(a[name], b[name])
+    assert torch.equal(far["key_pages"], want["key_pages"]) and (far["out"].float() - want["out"].float()).norm() <= 2.0 ** -8 * want["out"].float().norm()
+    last = int(np.argmax([n + s for n, s in zip(lens, starts)]))
+    row = int(c.row_starts[last + 1]) - 1
+    assert (less["out"][row] == 0).all() and torch.equal(less["out"][:row], b["out"][:row])
+    slot = starts[last] + lens[last] - 1
+    page, off = int(c.table[last, slot // 16]), slot % 16
+    assert torch.equal(less["key_pages"][page, off].cpu(), c.keys[page, off])
+    for context in (0, -1, room + 1):
+        with pytest.raises(ValueError):
+            large.run(**dict(c.device(), cos=cos, sin=sin, page_tables=table, context=context))
