@@ -245,21 +245,20 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         for (int q = 0; q < kTiles; ++q) sum_slot[q] = -1;
         fence_barrier_init();
     }
+    pdl_launch_dependents();
+    pdl_wait();   // queries, cache rows and lists come from the kernels before this one
+    const ChunkBlock blk = p.blocks[y];
+    if (blk.b < 0) return;   // no rows for this CTA, and none for the others of its cluster
+    // Tensor memory only now: a CTA that held it while it waited for the kernels before could keep it from one of them, which would wait
+    // for ever where the two and a third that has it for the moment share an SM.
     if (warp == S::load_warp) {
         tmem_alloc(tmem_slot, S::cols);
         tmem_relinquish();
     }
-    pdl_launch_dependents();
-    pdl_wait();   // queries, cache rows and lists come from the kernels before this one
-    const ChunkBlock blk = p.blocks[y];
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    if (blk.b < 0) {   // no rows for this CTA, and none for the others of its cluster
-        if (warp == S::load_warp) tmem_dealloc(tmem_base, S::cols);
-        return;
-    }
     // keys that a tile's last row sees, and the steps of this CTA
     int ends[kTiles], steps[kTiles], most = 0;
 #pragma unroll
