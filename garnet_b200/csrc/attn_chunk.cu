@@ -39,7 +39,7 @@ constexpr int kRowThreads = 128;
 
 // One CTA beside the rows': the attention's blocks of rows by the keys that they see, the most first, so that the last CTAs to start
 // are short ones (24 ragged sequences of 5 rows at up to 3500: 45 instead of 65 us, a ragged batch of 8 prompts 58 instead of 74 us with
-// the sequences in their own order).  A counting sort; blocks that see equally much (within 1 / 511 of max_context) come in any order.
+// the sequences in their own order, before weights entered as two numbers).  A counting sort; blocks that see equally much (within 1 / 511 of max_context) come in any order.
 constexpr int kOrderBuckets = 4 * kRowThreads;
 __device__ __forceinline__ void chunk_order(const Chunk& p)
 {

@@ -16,13 +16,15 @@
 // Few rows after a long context: a cluster of up to 8 CTAs shares the keys; every CTA sends its part of row i to CTA i % splits by
 // stores to distributed shared memory, which joins and writes it (launch_plan.h says when).
 //
-// Bound: a step of two tiles costs 1024 clocks of the exponential unit (16 per clock) and 1330 of the tensor pipe (N = 64 takes 50
-// clocks per MMA instead of 33: both operands come from shared memory); it takes 1800 (0.95 us): scores -> maximum -> exponentials
-// (780 clocks a tile, one tile after the other) -> P V is a chain.  B200, 16 / 8 heads, norms and cache append included: a prompt of
-// 8192 tokens 272 us (0.61 of the measured bf16 peak over the visible pairs), 512 tokens at 30000 128 us (0.60), a prompt of 2048
-// 42 us, 24 x 5 tokens at up to 3500 45 us (0.65 of the measured bandwidth), 4 tokens at 1000 10.0 us.  Steps of 128 keys with one
-// set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192 registers to a softmax thread) took 293 to 300 us
-// for 8192 tokens where these took 286; part of the exponentials as polynomials, and two softmax threads per row and tile, were no faster either.
+// Bound: a step of two tiles costs 1860 clocks of the tensor pipe (N = 64 takes 50 clocks per MMA of Q K^T instead of 33, since both
+// operands come from shared memory; P V, twice for a weight's two numbers, 66) and 1024 of the exponential unit (16 per clock); it takes
+// 2100 to 2350 (1.07 to 1.20 us): one tile's scores -> maximum -> exponentials -> two numbers beside the MMAs of the other.  B200, 16 / 8
+// heads, norms and cache append included, at 1965 MHz: a prompt of 8192 tokens 350 us (0.47 of the measured bf16 peak over the visible
+// pairs), 512 tokens at 30000 166 us (0.46), a prompt of 2048 46 us, 24 x 5 tokens at up to 3500 51 us (0.59 of the measured bandwidth), 4
+// tokens at 1000 11 us.  Call after call the power limit takes the clock down to 1590 MHz: 410 and 191 us for the two long ones.
+// With one number per weight, steps of 128 keys with one set of scores (MMAs of N = 128, P handed over in pieces of 32 keys, 128 or 192
+// registers to a softmax thread) took 293 to 300 us for 8192 tokens where these took 286; part of the exponentials as polynomials, and
+// two softmax threads per row and tile, were no faster either.
 // Numerics: q, k and v are bf16 (exact products), scores, statistics and sums fp32.  The tensor core cuts towards zero what it adds to a
 // sum: O is taken out of tensor memory every kChSumSteps steps and added in fp32, in memory of the workspace (19 MB, which stay in L2)
 // of which a tile holds a slot while it runs.  A weight of P meets V as two bf16 numbers, its first bits and the rest: 2^-15 of it is lost

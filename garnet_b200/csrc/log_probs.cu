@@ -15,9 +15,11 @@
 // Everything is added in an order that depends on sizes only.  A row whose maximum lies beyond +-2^100 (a mask of the type's lowest
 // value over all of it) or, in y, beyond +-2^20 (a temperature next to zero) is summed again, value by value, against its maximum.
 //
-// Bound: HBM in principle (every logit once).  For 16-bit logits the exponentials, 16 per clock and SM, take nearly as long (69 of 95 us for
-// 2048 rows of 151936): that call takes 125 us, 0.76 of the measured bandwidth, the exponential unit busy 64 % of it.  One row of 151936 and
-// 64 rows of 32003 fp32 take 11.5 us each, the latency of launch, loads, two meetings of the cluster and the alternatives' order.
+// Bound: HBM in principle (every logit once).  For 16-bit logits the exponentials, 16 per clock and SM, take nearly as long: 67 us of the
+// unit at 1965 MHz for 2048 rows of 151936 bf16, beside 95 us of the measured bandwidth.  That call takes 127 us (0.75 of the bandwidth; a
+// profiled launch of 126 us at its own clock counted the unit, with all that goes through it, busy for 64 %), fp16 130 us (its values
+// are converted and bounded one by one), 1024 rows of fp32 108 us (0.88).  One row of 151936 and 64 rows of 32003 fp32 take 11.5 us each,
+// the latency of launch, loads, two meetings of the cluster and the alternatives' order.
 #include <cfloat>
 #include <cmath>
 #include <cooperative_groups.h>
