@@ -10,9 +10,9 @@
 //   MMA warps       one thread per tile: P V of step u - 2, then the scores of step u into the set that its P leaves;
 //   scout warps     one per tile: wait for the MMAs' barrier in shared memory and pass it on to a named one;
 //   softmax warps   one thread per query row: scores into registers, running maximum, p = 2^(s c - m c), the row's sum in fp32, P as
-//                   two bf16 numbers each over the scores in tensor memory; O stays in tensor memory and is rescaled only when a row's maximum has
-//                   grown by more than 2^8 since the last time (the final division makes that exact).  The fp32 work runs two
-//                   values per instruction.  Two tiles take turns with their exponentials.
+//                   two bf16 numbers each over the scores in tensor memory; O stays in tensor memory for kChSumSteps steps and is
+//                   rescaled only when a row's maximum has grown by more than 2^8 since the last time (the final division makes that
+//                   exact).  The fp32 work runs two values per instruction.  Two tiles take turns with their exponentials.
 // Few rows after a long context: a cluster of up to 8 CTAs shares the keys; every CTA sends its part of row i to CTA i % splits by
 // stores to distributed shared memory, which joins and writes it (launch_plan.h says when).
 //
