@@ -247,12 +247,11 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
         for (int q = 0; q < kTiles; ++q) sum_slot[q] = -1;
         fence_barrier_init();
     }
-    pdl_launch_dependents();
     pdl_wait();   // queries, cache rows and lists come from the kernels before this one
     const ChunkBlock blk = p.blocks[y];
     if (blk.b < 0) return;   // no rows for this CTA, and none for the others of its cluster
-    // Tensor memory only now: a CTA that held it while it waited for the kernels before could keep it from one of them, which would wait
-    // for ever where the two and a third that has it for the moment share an SM.
+    // Tensor memory is taken behind the wait, and the kernels behind this one come up when all of its CTAs have theirs: a CTA that holds
+    // tensor memory while it waits for another kernel could keep it from that kernel's CTA on the same SM, and both would wait for ever.
     if (warp == S::load_warp) {
         tmem_alloc(tmem_slot, S::cols);
         tmem_relinquish();
@@ -260,6 +259,7 @@ __global__ void __launch_bounds__(ChShape<kTiles, kUnits>::threads, kUnits == 2 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch_dependents();
     const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // keys that a tile's last row sees, and the steps of this CTA
     int ends[kTiles], steps[kTiles], most = 0;

@@ -543,3 +543,32 @@ def test_a_call_that_says_how_far_its_rows_reach(lens, starts, heads):
     for context in (0, -1, room + 1):
         with pytest.raises(ValueError):
             large.run(**dict(c.device(), cos=cos, sin=sin, page_tables=table, context=context))
+
+
+@pytest.mark.parametrize("rows,start", [(96, 40), (5, 900)])
+def test_between_linears_that_use_tensor_memory_too(rows, start):
+    """Linear, attention, linear without a wait on the host, as the layers of a prompt follow one another: all three take tensor memory and may come
+    up before the kernels that they wait for are done."""
+    c = Case([rows], [start], 16, 8, seed=51)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    mk = lambda n, k: garnet_b200.W4A16Linear().prepare(*garnet_b200.quantize_int4(torch.randn(n, k, device="cuda", generator=gen) / 32), n, k)   # noqa: E731
+    qkv_lin, o_lin = mk(c.cfg.qkv_width, 1024), mk(1024, 2048)
+    x = torch.randn(rows, 1024, device="cuda", generator=gen).to(torch.bfloat16)
+    d, op = c.device(), c.op()
+    steps = []
+    for sync in (True, False):
+        y = x
+        for _ in range(12):
+            qkv = qkv_lin.forward(y)
+            if sync:
+                torch.cuda.synchronize()
+            out = torch.zeros(rows, 2048, dtype=torch.bfloat16, device="cuda")
+            op.run(**dict(d, qkv=qkv, out=out), pdl=not sync)
+            if sync:
+                torch.cuda.synchronize()
+            y = o_lin.forward(out)
+            if sync:
+                torch.cuda.synchronize()
+        steps.append(y)
+    torch.cuda.synchronize()
+    assert steps[0].isfinite().all() and torch.equal(steps[0], steps[1])
